@@ -255,6 +255,72 @@ int pinn_adam_step(float *theta, const float *grad, float *exp_avg, float *exp_a
                    int64_t n, float lr, double beta1, double beta2, float eps, float weight_decay,
                    int32_t decoupled, void *stream);
 
+/* ---- AdamW over many tensors, global gradient norm ----------------------------------------------------------
+ * What pinn_adam_step does for ONE flat float32 vector, for tensors that lie anywhere, of float32, bfloat16 or float16,
+ * with moments in float32 or in 8 bits, optional float32 master weights and clipping of the global gradient norm:
+ *   f = min(1, max_norm / (norm + 1e-6));  m = b1 m + (1 - b1) f g;  v = b2 v + (1 - b2) (f g)^2
+ *   p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
+ * Moments, master weights and scales are flat device buffers in which every tensor starts at a multiple of
+ * PINN_ADAMW_BLOCK elements (`offset` below); the elements behind a tensor's end are not written to (8 bits: they hold 0).
+ * 8-bit moments: one scale byte s per block, 2^(s - 127), 255 = the block holds a value that is not finite (it reads NaN
+ * from then on); exp_avg: sign, 4 bits of exponent (bias 7), 3 of mantissa; exp_avg_sq: 5 bits of exponent (bias 15), 3 of mantissa.
+ * They are rounded up or down by a sequence over steps and elements that is even on both sides; a positive v never becomes 0.
+ * No entry point here allocates or synchronises: all are graph-capturable.  pinn_adamw_group_step must not run twice at
+ * once on the same `ticket` (one optimizer, one stream).  The pointer arrays are HOST arrays of device pointers, read before the call returns. */
+#define PINN_F32 0
+#define PINN_BF16 1
+#define PINN_F16 2
+#define PINN_ADAMW_BLOCK 128         /* elements that share a scale */
+#define PINN_ADAMW_CHUNK 2048        /* elements per entry of chunk_tensor */
+#define PINN_ADAMW_MAX_TENSORS 240   /* tensors per call: their addresses are launch arguments */
+#define PINN_ADAMW_GRID 2048         /* most workgroups of a step */
+#define PINN_NORM_PARTIALS 1024      /* most partial sums per launch of pinn_grad_sumsq */
+
+typedef struct {
+    int64_t numel;
+    int64_t offset;                  /* first element in the flat buffers, a multiple of PINN_ADAMW_BLOCK */
+    int64_t first_chunk;             /* first entry in chunk_tensor */
+    int64_t row;                     /* row of device_state */
+} PinnTensorSpan;
+
+typedef struct {
+    const PinnTensorSpan *spans;     /* device, one per tensor of the call */
+    const uint16_t *chunk_tensor;    /* device: the tensor (0 .. n_tensors - 1) of each chunk, ceil(numel / PINN_ADAMW_CHUNK) per tensor, in order */
+    int64_t n_chunks;
+    int32_t n_tensors;
+    int32_t dtype;                   /* of parameters and gradients */
+    int32_t state_bits;              /* 32 or 8 */
+    int32_t skip_nonfinite;          /* with partials: a norm that is not finite leaves everything as it was */
+    void *exp_avg, *exp_avg_sq;      /* float32, or codes */
+    uint8_t *exp_avg_scale, *exp_avg_sq_scale;
+    float *master;                   /* NULL: none; else the weights that are updated, the parameters are their rounded copy */
+    double *device_state;            /* rows of step, beta1^step, beta2^step; zeros to start */
+    uint32_t *ticket;                /* zero to start; every call leaves it zero */
+    const double *partials;          /* from pinn_grad_sumsq, over the tensors that are clipped together */
+    int32_t n_partials;              /* 0: no norm */
+    int32_t reserved;
+    float *norm;                     /* NULL, or where the norm goes */
+    double max_norm;                 /* < 0: the norm is not used for clipping */
+    double lr, beta1, beta2, eps, weight_decay;
+} PinnAdamWGroup;
+
+/* one step of all tensors whose gradient is not NULL; their rows of device_state advance on the device */
+int pinn_adamw_group_step(const PinnAdamWGroup *group, void *const *params, const void *const *grads, void *stream);
+/* 8-bit moments as float32; n: length of the flat buffers, a multiple of PINN_ADAMW_BLOCK */
+int pinn_adamw_moments(const uint8_t *exp_avg, const uint8_t *exp_avg_sq, const uint8_t *exp_avg_scale,
+                       const uint8_t *exp_avg_sq_scale, float *exp_avg_out, float *exp_avg_sq_out, int64_t n, void *stream);
+
+/* partial sums of squares (float64) over a list of tensors; `partials`: device, room for `n_reserved` (pinn_grad_norm_partials
+ * of the list's length); *n_partials: how many were written.  The same inputs give the same bits. */
+int64_t pinn_grad_norm_partials(int32_t n_tensors);
+int pinn_grad_sumsq(const void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, double *partials,
+                    int64_t n_reserved, int32_t *n_partials, void *stream);
+/* *norm = sqrt of their sum */
+int pinn_grad_norm(const double *partials, int32_t n_partials, float *norm, void *stream);
+/* the same, and grads *= min(1, max_norm / (norm + 1e-6)) in place; no two tensors may overlap */
+int pinn_grad_clip(void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, const double *partials,
+                   int32_t n_partials, double max_norm, float *norm, void *stream);
+
 const char *pinn_error_string(int code);
 
 #define PINN_OK 0
@@ -264,6 +330,7 @@ const char *pinn_error_string(int code);
 #define PINN_ERR_NULL (-4)
 #define PINN_ERR_ALLOC (-5)
 #define PINN_ERR_TOO_LARGE (-6)
+#define PINN_ERR_OVERLAP (-7)
 
 #ifdef __cplusplus
 }

@@ -27,6 +27,25 @@ class PinnDesc(ctypes.Structure):
     ]
 
 
+class PinnTensorSpan(ctypes.Structure):
+    _fields_ = [("numel", ctypes.c_int64), ("offset", ctypes.c_int64), ("first_chunk", ctypes.c_int64), ("row", ctypes.c_int64)]
+
+
+class PinnAdamWGroup(ctypes.Structure):
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("spans", "chunk_tensor")] + [("n_chunks", ctypes.c_int64)]
+                + [(k, ctypes.c_int32) for k in ("n_tensors", "dtype", "state_bits", "skip_nonfinite")]
+                + [(k, ctypes.c_void_p) for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master",
+                                                  "device_state", "ticket", "partials")]
+                + [("n_partials", ctypes.c_int32), ("reserved", ctypes.c_int32), ("norm", ctypes.c_void_p)]
+                + [(k, ctypes.c_double) for k in ("max_norm", "lr", "beta1", "beta2", "eps", "weight_decay")])
+
+
+# include/pinnjet.h: dtype codes and the constants of the AdamW step over many tensors
+DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_TENSORS = 128, 2048, 240
+ERR_OVERLAP = -7
+
+
 class NativeError(RuntimeError):
     pass
 
@@ -42,6 +61,7 @@ SYMBOLS = [
     "pinn_lbfgs_workspace_floats", "pinn_lbfgs_direction", "pinn_lbfgs_eval_stats",
     "pinn_lbfgs_direction_advance", "pinn_lbfgs_eval_stats_keep", "pinn_host_device_pointer",
     "pinn_lbfgs_poll_advance",
+    "pinn_adamw_group_step", "pinn_adamw_moments", "pinn_grad_norm_partials", "pinn_grad_sumsq", "pinn_grad_norm", "pinn_grad_clip",
 ]
 
 
@@ -83,6 +103,13 @@ def load_library():
     lib.pinn_data_loss.argtypes = [vp, vp, i32, i32, i32, i32, vp, vp]
     lib.pinn_data_loss_cotangent.argtypes = [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp]
     lib.pinn_closure_sum.argtypes = [vp, i32, vp, i32, f32, vp, vp, vp, vp, i64, i32, vp]
+    lib.pinn_adamw_group_step.argtypes = [ctypes.POINTER(PinnAdamWGroup), vp, vp, vp]
+    lib.pinn_adamw_moments.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp]
+    lib.pinn_grad_norm_partials.argtypes = [i32]
+    lib.pinn_grad_norm_partials.restype = i64
+    lib.pinn_grad_sumsq.argtypes = [vp, vp, vp, i32, vp, i64, ctypes.POINTER(i32), vp]
+    lib.pinn_grad_norm.argtypes = [vp, i32, vp, vp]
+    lib.pinn_grad_clip.argtypes = [vp, vp, vp, i32, vp, i32, ctypes.c_double, vp, vp]
     lib.pinn_error_string.argtypes = [ctypes.c_int]
     lib.pinn_error_string.restype = ctypes.c_char_p
     _lib = lib

@@ -524,6 +524,7 @@ const char *pinn_error_string(int code)
     case PINN_ERR_NULL: return "null pointer";
     case PINN_ERR_ALLOC: return "device allocation failed";
     case PINN_ERR_TOO_LARGE: return "problem too large for the static scratch of the no-allocation entry point";
+    case PINN_ERR_OVERLAP: return "two tensors share memory";
     default: return "unknown error";
     }
 }

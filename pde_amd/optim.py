@@ -4,13 +4,20 @@ The reference's Adam phase is `torch.optim.Adam(self.dnn.parameters())` / `AdamW
 (7kdv/PI-7kdv3soliton.py:138,154-157; 7kdv/sw73-adamW.py:170): ten parameter tensors, ~15 foreach launches per
 step.  `FusedAdam` has the same constructor arguments, the same update rule (torch's default, non-amsgrad
 Adam; `decoupled=True` is AdamW) and the usual `zero_grad()` / `step()` protocol; the step count lives on the
-device, so a captured HIP graph replays it as is.  There is no CPU fallback: it needs libpinnjet.so and a GPU.
+device, so a captured HIP graph replays it as is.
+
+`GroupedAdamW` is the step for everything else: tensors that lie anywhere, several parameter groups, bfloat16 and float16
+weights, moments in 32 or 8 bits, clipping of the global gradient norm; `grad_norm` and `clip_grad_norm_` are that norm alone.
+
+There is no CPU fallback: all of it needs libpinnjet.so and a GPU.
 """
 import ctypes
 
+import numpy as np
 import torch
 
-from ._native import NativeError, _check, load_library
+from ._native import (ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_TENSORS, DTYPE_CODES, ERR_OVERLAP, NativeError, PinnAdamWGroup, _check, _cur_stream,
+                      _on, load_library)
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -121,4 +128,333 @@ class FusedAdam(torch.optim.Optimizer):
                                            float(grp["eps"]), float(grp["weight_decay"]), 1 if grp["decoupled"] else 0,
                                            ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)),
                    "pinn_adam_step")
+        return loss
+
+
+def _flat(t):
+    """`t`'s elements in the order in which they lie in memory, as a 1-D view; None where they have gaps or overlap."""
+    if not t.is_contiguous():
+        expect = 1
+        for size, stride in sorted(zip(t.shape, t.stride()), key=lambda x: (x[1], x[0])):
+            if size != 1 and stride != expect:
+                return None
+            expect *= size
+    return t.as_strided((t.numel(),), (1,), t.storage_offset())
+
+
+class _GradList:
+    """Gradients as the C interface takes them: host arrays of addresses, lengths and types."""
+
+    def __init__(self, grads, device, writable):
+        n = len(grads)
+        self.n, self.device, self.back, keep = n, device, [], []
+        codes = DTYPE_CODES
+        ptr, numel, dtype = [], [], []
+        for g in grads:
+            if g.layout is not torch.strided or g.dtype not in codes:
+                raise ValueError("gradients are dense float32, bfloat16 or float16 tensors, got %s, %s" % (g.layout, g.dtype))
+            if g.device != device:
+                raise ValueError("all gradients lie on one device, got %s and %s" % (device, g.device))
+            if not g.is_contiguous() and _flat(g) is None:
+                if writable and any(st == 0 and sz > 1 for sz, st in zip(g.shape, g.stride())):
+                    raise ValueError("a gradient that was expanded cannot be scaled in place")
+                c = g.contiguous()
+                self.back.append((g, c))
+                g = c
+            keep.append(g)
+            ptr.append(g.data_ptr())
+            numel.append(g.numel())
+            dtype.append(codes[g.dtype])
+        self.keep = keep
+        self.ptr, self.numel, self.dtype = (ctypes.c_uint64 * n)(*ptr), (ctypes.c_int64 * n)(*numel), (ctypes.c_int32 * n)(*dtype)
+
+    def sumsq(self, stream):
+        """(partial sums, how many): the workspace is this call's own"""
+        lib = load_library()
+        room = lib.pinn_grad_norm_partials(self.n)
+        partials = torch.empty(max(1, room), dtype=torch.float64, device=self.device)
+        count = ctypes.c_int32()
+        _check(lib.pinn_grad_sumsq(self.ptr, self.numel, self.dtype, self.n, partials.data_ptr(), room, ctypes.byref(count), stream), "pinn_grad_sumsq")
+        return partials, count.value
+
+
+def _tensor_list(tensors):
+    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
+    for t in tensors:
+        if not torch.is_tensor(t):
+            raise TypeError("expected tensors, got %s" % type(t).__name__)
+    if tensors and not tensors[0].is_cuda:
+        raise NativeError("the tensors are on %s: pde_amd needs an AMD GPU; there is no CPU fallback" % tensors[0].device)
+    return tensors
+
+
+@torch.no_grad()
+def grad_norm(tensors):
+    """2-norm over all elements of all `tensors` (one, or an iterable; float32, bfloat16, float16, mixed as they come): a 0-dim
+    float32 tensor on their device.  Squares and sums are float64, in a fixed order: the same inputs give the same bits, and
+    no float32 value overflows or vanishes on the way.  An empty list gives 0."""
+    tensors = _tensor_list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    dev = tensors[0].device
+    lst = _GradList(tensors, dev, writable=False)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    with _on(dev):
+        stream = _cur_stream(norm)
+        partials, n = lst.sumsq(stream)
+        _check(load_library().pinn_grad_norm(partials.data_ptr(), n, norm.data_ptr(), stream), "pinn_grad_norm")
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+    """Scales the gradients of `parameters` in place so that their global 2-norm is at most `max_norm`, and returns the norm
+    they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 160 tensors, without a copy of the
+    gradients.  The factor is min(1, max_norm / (norm + 1e-6)); with a norm that is not finite it is 0 or NaN, as there;
+    `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError)."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("max_norm is %r: 0 or more is needed" % max_norm)
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = _tensor_list([p.grad for p in parameters if p.grad is not None])
+    if not grads:
+        return torch.tensor(0.0)
+    dev = grads[0].device
+    lst = _GradList(grads, dev, writable=True)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    lib = load_library()
+    with _on(dev):
+        stream = _cur_stream(norm)
+        partials, n = lst.sumsq(stream)
+        if error_if_nonfinite:
+            _check(lib.pinn_grad_norm(partials.data_ptr(), n, norm.data_ptr(), stream), "pinn_grad_norm")
+            if not torch.isfinite(norm):
+                raise RuntimeError("the gradients' norm is %s: they were not clipped" % norm.item())
+        rc = lib.pinn_grad_clip(lst.ptr, lst.numel, lst.dtype, lst.n, partials.data_ptr(), n, max_norm, norm.data_ptr(), stream)
+        if rc == ERR_OVERLAP:
+            raise ValueError("two of the gradients share memory: scaling them in place would scale it twice")
+        _check(rc, "pinn_grad_clip")
+        for g, c in lst.back:
+            g.copy_(c)
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+class GroupedAdamW(torch.optim.Optimizer):
+    """AdamW over many tensors at once: one launch per 240 tensors of one group and type.
+
+    torch.optim.AdamW's constructor arguments and update rule (decoupled weight decay, no amsgrad; `weight_decay=0` is Adam), plus
+
+    state_bits      32: moments in float32.  8: one byte each, in blocks of 128 elements with a power-of-two scale (2 1/64 bytes
+                    per weight instead of 8): exp_avg keeps 4 significant bits and a range of 2^17 in a block, exp_avg_sq 4 bits and 2^33;
+                    rounded by an even sequence, so that small changes are not lost.  A gradient that is not finite makes its whole block's moments NaN.
+    max_norm        clip the gradients' global 2-norm (over all groups, tensors without a gradient left out) inside the step; the gradients themselves
+                    stay as they are.  `grad_norm` holds the norm of the last step, on the device.
+    skip_nonfinite  a step whose gradient norm is not finite changes nothing, counters included (decided on the device).
+    master_weights  bfloat16 and float16 parameters are the rounded copy of float32 weights held here (`master`); after writing to
+                    such a parameter from outside call `sync_master()`.
+
+    Parameters are dense float32, bfloat16 or float16 CUDA tensors on one device that do not share memory, in any number of groups;
+    gradients have their parameter's type.  A parameter whose `.grad` is None is left alone and its step count with it.  Step counts and powers of beta
+    live on the device (`device_state`), so a captured step replays; learning rates and the like are taken at the call.
+    After a change of betas the bias correction takes the product of the betas that were used.
+
+    Moments lie in flat buffers in the order of the parameters, each at the next multiple of 128 elements, in the order its
+    parameter has in memory: `moments()`."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None, skip_nonfinite=False,
+                 master_weights=False):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits is %r: 8 or 32 is needed" % (state_bits,))
+        if max_norm is not None and not float(max_norm) >= 0.0:
+            raise ValueError("max_norm is %r: 0 or more is needed" % (max_norm,))
+        self.state_bits, self.max_norm, self.skip_nonfinite = state_bits, None if max_norm is None else float(max_norm), bool(skip_nonfinite)
+        self._planned = False
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        for grp in self.param_groups:
+            self._hyper(grp)
+        self._params = [p for grp in self.param_groups for p in grp["params"]]
+        self.device = self._params[0].device
+        if self.device.type != "cuda":
+            raise NativeError("GroupedAdamW needs parameters on an AMD GPU, got %s; there is no CPU fallback (use torch.optim.AdamW)" % self.device)
+        self._check_params()
+        self.lib = load_library()
+        self._plan(bool(master_weights))
+        self._planned = True
+
+    def add_param_group(self, param_group):
+        if self._planned:
+            raise ValueError("GroupedAdamW takes all parameter groups when it is made")
+        super().add_param_group(param_group)
+
+    @staticmethod
+    def _hyper(grp):
+        lr, (b1, b2), eps, wd = float(grp["lr"]), grp["betas"], float(grp["eps"]), float(grp["weight_decay"])
+        if not (lr >= 0.0 and eps >= 0.0 and wd >= 0.0 and 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError("lr %r, betas %r, eps %r, weight_decay %r: none may be negative, betas are below 1"
+                             % (grp["lr"], grp["betas"], grp["eps"], grp["weight_decay"]))
+        return lr, float(b1), float(b2), eps, wd
+
+    def _check_params(self):
+        spans = []
+        for i, p in enumerate(self._params):
+            if p.layout is not torch.strided or p.dtype not in DTYPE_CODES:
+                raise ValueError("parameter %d is %s, %s: dense float32, bfloat16 or float16 is needed" % (i, p.layout, p.dtype))
+            if p.device != self.device:
+                raise ValueError("parameters lie on one device, got %s and %s" % (self.device, p.device))
+            if _flat(p) is None:
+                raise ValueError("parameter %d (shape %s, strides %s) has gaps or overlaps in memory" % (i, tuple(p.shape), p.stride()))
+            if p.numel():
+                spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+        spans.sort()
+        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+            raise ValueError("two parameters share memory")
+
+    def _plan(self, master_weights):
+        """Flat state, and the device tables of each launch."""
+        dev, at = self.device, 0
+        self.offsets = []
+        for p in self._params:
+            self.offsets.append(at)
+            at += -(-p.numel() // ADAMW_BLOCK) * ADAMW_BLOCK
+        self.state_numel = at
+        kind = torch.float32 if self.state_bits == 32 else torch.uint8
+        self.exp_avg, self.exp_avg_sq = (torch.zeros(at, dtype=kind, device=dev) for _ in range(2))
+        self.exp_avg_scale = self.exp_avg_sq_scale = self.master = None
+        if self.state_bits == 8:
+            self.exp_avg_scale, self.exp_avg_sq_scale = (torch.zeros(at // ADAMW_BLOCK, dtype=torch.uint8, device=dev) for _ in range(2))
+        if master_weights and any(p.dtype != torch.float32 for p in self._params):
+            self.master = torch.zeros(at, dtype=torch.float32, device=dev)
+            self.sync_master()
+        self.device_state = torch.zeros((len(self._params), 3), dtype=torch.float64, device=dev)   # step, beta1^step, beta2^step
+        self._ticket = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._norm = torch.zeros((), dtype=torch.float32, device=dev)
+        self._launches, first = [], 0
+        for grp in self.param_groups:
+            rows = range(first, first + len(grp["params"]))
+            first += len(grp["params"])
+            for dt in DTYPE_CODES:
+                mine = [i for i in rows if self._params[i].dtype == dt and self._params[i].numel()]
+                for a in range(0, len(mine), ADAMW_MAX_TENSORS):
+                    self._launches.append(self._launch(grp, dt, mine[a:a + ADAMW_MAX_TENSORS]))
+
+    def _launch(self, grp, dtype, rows):
+        spans, chunks, at = [], [], 0
+        for k, i in enumerate(rows):
+            n = self._params[i].numel()
+            count = -(-n // ADAMW_CHUNK)
+            spans.append((n, self.offsets[i], at, i))
+            chunks.append(np.full(count, k, dtype=np.uint16))
+            at += count
+        spans = torch.from_numpy(np.array(spans, dtype=np.int64)).to(self.device)
+        chunks = torch.from_numpy(np.concatenate(chunks).view(np.int16)).to(self.device)
+        d = PinnAdamWGroup()
+        d.spans, d.chunk_tensor, d.n_chunks, d.n_tensors = spans.data_ptr(), chunks.data_ptr(), at, len(rows)
+        d.dtype, d.state_bits, d.skip_nonfinite = DTYPE_CODES[dtype], self.state_bits, int(self.skip_nonfinite)
+        d.exp_avg, d.exp_avg_sq, d.device_state, d.ticket = (t.data_ptr() for t in (self.exp_avg, self.exp_avg_sq, self.device_state, self._ticket))
+        if self.state_bits == 8:
+            d.exp_avg_scale, d.exp_avg_sq_scale = self.exp_avg_scale.data_ptr(), self.exp_avg_sq_scale.data_ptr()
+        if self.master is not None and dtype != torch.float32:
+            d.master = self.master.data_ptr()
+        d.max_norm = -1.0 if self.max_norm is None else self.max_norm
+        return dict(grp=grp, desc=d, rows=rows, p=(ctypes.c_uint64 * len(rows))(), g=(ctypes.c_uint64 * len(rows))(), tables=(spans, chunks))
+
+    @torch.no_grad()
+    def sync_master(self):
+        """The float32 weights take the parameters' present values."""
+        if self.master is None:
+            return
+        for p, at in zip(self._params, self.offsets):
+            self.master[at:at + p.numel()].copy_(_flat(p))
+
+    @property
+    def grad_norm(self):
+        """norm of the gradients of the last step (0-dim float32, overwritten by the next); steps without `max_norm` or `skip_nonfinite` do not form it"""
+        return self._norm
+
+    @torch.no_grad()
+    def moments(self):
+        """(exp_avg, exp_avg_sq) as flat float32 tensors in the order of the flat state: the buffers themselves, or with 8 bits what they stand for."""
+        if self.state_bits == 32:
+            return self.exp_avg, self.exp_avg_sq
+        m, v = (torch.empty(self.state_numel, dtype=torch.float32, device=self.device) for _ in range(2))
+        with _on(self.device):
+            _check(self.lib.pinn_adamw_moments(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr(),
+                                               self.exp_avg_sq_scale.data_ptr(), m.data_ptr(), v.data_ptr(), self.state_numel, _cur_stream(m)),
+                   "pinn_adamw_moments")
+        return m, v
+
+    def _held(self):
+        names = ["exp_avg", "exp_avg_sq", "device_state"]
+        names += ["exp_avg_scale", "exp_avg_sq_scale"] if self.state_bits == 8 else []
+        return names + (["master"] if self.master is not None else [])
+
+    def state_dict(self):
+        """torch's layout plus `fused`: the flat state, types preserved."""
+        sd = super().state_dict()
+        sd["fused"] = {name: getattr(self, name).clone() for name in self._held()}
+        return sd
+
+    def load_state_dict(self, state_dict):
+        sd = dict(state_dict)
+        fused = sd.pop("fused", None)
+        if fused is not None:
+            if sorted(fused) != sorted(self._held()):
+                raise ValueError("GroupedAdamW.load_state_dict: the state has %s, expected %s" % (sorted(fused), sorted(self._held())))
+            for name in self._held():
+                dst, src = getattr(self, name), fused[name]
+                if src.shape != dst.shape or src.dtype != dst.dtype:
+                    raise ValueError("GroupedAdamW.load_state_dict: %s is %s %s, expected %s %s"
+                                     % (name, tuple(src.shape), src.dtype, tuple(dst.shape), dst.dtype))
+        super().load_state_dict(sd)
+        first = 0
+        for grp in self.param_groups:                   # torch has replaced the groups' dicts
+            for launch in self._launches:
+                if first <= launch["rows"][0] < first + len(grp["params"]):
+                    launch["grp"] = grp
+            first += len(grp["params"])
+        if fused is not None:
+            for name in self._held():
+                getattr(self, name).copy_(fused[name])
+
+    def _gradient(self, p):
+        """`p.grad` in `p`'s order in memory"""
+        g = p.grad
+        if g.layout is not torch.strided:
+            raise ValueError("GroupedAdamW takes dense gradients, got %s" % g.layout)
+        if g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+            raise ValueError("the gradient is %s %s on %s, its parameter %s %s on %s" % (tuple(g.shape), g.dtype, g.device, tuple(p.shape), p.dtype, p.device))
+        if g.stride() != p.stride():
+            g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+        return g
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        params, grads = self._params, []
+        for i, p in enumerate(params):
+            if p.grad is None:
+                grads.append(None)
+                continue
+            grads.append(self._gradient(p))
+        hyper = {id(grp): self._hyper(grp) for grp in self.param_groups}
+        given = [g for g in grads if g is not None and g.numel()]
+        if not given:
+            return loss
+        with _on(self.device):
+            stream = _cur_stream(self._norm)
+            partials, n_partials = None, 0
+            if self.max_norm is not None or self.skip_nonfinite:
+                partials, n_partials = _GradList(given, self.device, writable=False).sumsq(stream)
+            for launch in self._launches:
+                d, rows = launch["desc"], launch["rows"]
+                launch["p"][:] = [params[i].data_ptr() for i in rows]
+                launch["g"][:] = [0 if grads[i] is None else grads[i].data_ptr() for i in rows]
+                d.lr, d.beta1, d.beta2, d.eps, d.weight_decay = hyper[id(launch["grp"])]
+                d.partials, d.n_partials, d.norm = partials.data_ptr() if n_partials else None, n_partials, self._norm.data_ptr()
+                _check(self.lib.pinn_adamw_group_step(ctypes.byref(d), launch["p"], launch["g"], stream), "pinn_adamw_group_step")
+        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
         return loss

@@ -83,7 +83,10 @@ class PhysicsInformedNN:
     overlap_streams = None
     closure_impl = "direct"          # backward(): "direct" (no autograd graph, see _loss_terms_direct) or "autograd"
     hip_graph_fallback = False       # a failed capture raises; True: report it and continue with the eager loop
-    adam_impl = "fused"              # "fused": pde_amd.optim.FusedAdam (one launch per step); "torch": torch.optim.Adam/AdamW
+    adam_impl = "fused"              # "fused": pde_amd.optim.FusedAdam (one launch per step); "torch": torch.optim.Adam/AdamW;
+                                     # "grouped": pde_amd.optim.GroupedAdamW, with the two options below
+    adam_state_bits = 32             # "grouped": moments in float32 (32) or one byte each (8)
+    max_grad_norm = None             # "grouped": clip the gradient's 2-norm inside every Adam step
     lbfgs_impl = "device"            # "device": pde_amd.lbfgs.LBFGS (three launches per direction, csrc/lbfgs.hip); "torch": torch.optim.LBFGS
     shard_loss1_min_rows = 4096      # sharded runs: a bc class's loss1 grid of at least this many rows is sharded over the ranks
     lbfgs_kernels_factory = None     # test hook: callable(n, history) -> stand-in for the L-BFGS launches
@@ -685,7 +688,13 @@ class PhysicsInformedNN:
         self.iter = init_iter
         params = list(self.dnn.parameters())
         self._fused_adam = self.adam_impl == "fused" and torch.device(self.device).type == "cuda"
-        if self._fused_adam:
+        if self.adam_impl != "grouped" and (self.max_grad_norm is not None or self.adam_state_bits != 32):
+            raise ValueError('max_grad_norm and adam_state_bits need adam_impl = "grouped", this is "%s"' % self.adam_impl)
+        if self.adam_impl == "grouped":
+            from .optim import GroupedAdamW
+            self.optimizer_Adam = GroupedAdamW(params, weight_decay=v.weight_decay if v.optimizer == "adamw" else 0.0,
+                                               state_bits=self.adam_state_bits, max_norm=self.max_grad_norm)
+        elif self._fused_adam:
             # same update rule and defaults as torch.optim.Adam / AdamW(weight_decay=1e-2), one launch per step
             from .optim import FusedAdam
             self.optimizer_Adam = FusedAdam(params, flat_params=self.dnn.flat_theta(), decoupled=v.optimizer == "adamw",
@@ -761,7 +770,7 @@ class PhysicsInformedNN:
         and step count of the warm-up iterations are kept."""
         v = self.variant
         kw = dict(capturable=True)
-        if self._fused_adam:
+        if self._fused_adam or self.adam_impl == "grouped":
             opt = self.optimizer_Adam            # its step count lives on the device: capturable as it is
         elif v.optimizer == "adamw":
             opt = torch.optim.AdamW(params, weight_decay=v.weight_decay, **kw)

@@ -1,0 +1,146 @@
+"""CPU: what GroupedAdamW, grad_norm, clip_grad_norm_ and their C entries refuse before anything reaches a GPU, and the float64
+formulas the GPU tests use (adamw_formulas.py) against torch.optim.AdamW and against the 8-bit format's own properties."""
+import ctypes
+import os
+
+import numpy as np
+import pytest
+import torch
+
+import adamw_formulas as F
+from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_TENSORS, NativeError, PinnAdamWGroup, PinnTensorSpan, load_library
+from pde_amd.optim import GroupedAdamW, clip_grad_norm_, grad_norm
+from conftest import GOLDEN, ROOT
+
+needs_lib = pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="libpinnjet.so not built")
+
+
+def test_formulas_follow_torch():
+    """float64 against float64: three steps of torch.optim.AdamW, 1e-14 of |p| + lr for the few roundings of each"""
+    torch.manual_seed(0)
+    p = torch.nn.Parameter(torch.randn(50, dtype=torch.float64))
+    opt = torch.optim.AdamW([p], lr=1e-2, weight_decay=0.1)
+    q, m, v = p.detach().numpy().copy(), np.zeros(50), np.zeros(50)
+    for t in range(1, 4):
+        p.grad = torch.randn(50, dtype=torch.float64)
+        opt.step()
+        q, m, v = F.step(q, p.grad.numpy(), m, v, t, lr=1e-2, wd=0.1)
+        assert np.abs(p.detach().numpy() - q).max() < 1e-14 * (np.abs(q).max() + 1e-2)
+
+
+@pytest.mark.parametrize("form", [F.M, F.V])
+def test_eight_bit_format(form):
+    rng = np.random.default_rng(1)
+    tab = F.table(form)
+    assert len(tab) == form["codes"] and (np.diff(tab) > 0).all() and tab[-1] == 1.75 * 2.0 ** (15 - form["bias"] if form is F.M else 31 - form["bias"])
+    x = rng.standard_normal(128) * np.exp(3 * rng.standard_normal(128))
+    x = np.abs(x) if form is F.V else x
+    up = 0
+    for t in range(64):
+        y, s = F.round_block(x, 256, t, form)
+        step = np.maximum(np.abs(x) / 8, tab[1] * 2.0 ** (s - 127))            # between codes: 3 bits, below the normals the smallest code
+        assert (np.abs(y - x) <= step * (1 + 1e-12)).all()                     # a whole step at most, either way
+        assert np.array_equal(F.round_block(y, 256, t, form)[0], y)            # what is on a code stays
+        up += y - x
+    assert (np.abs(up / 64) <= step * 4 / 64).all()                            # an even sequence: within 4 of 64 places
+    y, s = F.round_block(np.zeros(128), 0, 1, form)
+    assert s == 0 and not y.any()
+    assert F.round_block(np.full(128, np.inf), 0, 1, form)[1] == 255
+    if form is F.V:
+        tiny = np.full(128, 1e-60)
+        tiny[0] = 1.0
+        assert (F.round_block(tiny, 0, 1, form)[0] > 0).all()
+
+
+def test_refusals_without_a_gpu():
+    p = torch.nn.Parameter(torch.ones(3))
+    with pytest.raises(NativeError, match="no CPU fallback"):
+        GroupedAdamW([p])
+    for kw, word in ((dict(state_bits=16), "state_bits"), (dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm"),
+                     (dict(lr=-1.0), "lr"), (dict(betas=(1.0, 0.9)), "betas"), (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=-1e-8), "eps"),
+                     (dict(weight_decay=-1.0), "weight_decay"), (dict(lr=float("nan")), "lr")):
+        with pytest.raises(ValueError, match=word):
+            GroupedAdamW([p], **kw)
+    with pytest.raises(ValueError):
+        GroupedAdamW([])
+    p.grad = torch.ones(3)
+    with pytest.raises(NativeError, match="no CPU fallback"):
+        clip_grad_norm_(p, 1.0)
+    with pytest.raises(NativeError, match="no CPU fallback"):
+        grad_norm([p.grad])
+    with pytest.raises(ValueError, match="max_norm"):
+        clip_grad_norm_(p, -0.5)
+    with pytest.raises(TypeError):
+        grad_norm([3.0])
+
+
+@needs_lib
+def test_c_entries_refuse_without_a_gpu():
+    lib = load_library()
+    header = open(os.path.join(ROOT, "include", "pinnjet.h")).read()
+    for name, value in (("PINN_ADAMW_BLOCK", ADAMW_BLOCK), ("PINN_ADAMW_CHUNK", ADAMW_CHUNK), ("PINN_ADAMW_MAX_TENSORS", ADAMW_MAX_TENSORS)):
+        assert "#define %s %d " % (name, value) in header
+    assert ctypes.sizeof(PinnTensorSpan) == 32 and ctypes.sizeof(PinnAdamWGroup) == 168
+    one = (ctypes.c_uint64 * 2)(4096, 8192)
+    INVALID, NULL, LARGE, OVERLAP = -1, -4, -6, -7
+
+    def group(**kw):
+        d = PinnAdamWGroup(n_tensors=2, n_chunks=2, dtype=0, state_bits=32, spans=16, chunk_tensor=16, exp_avg=16, exp_avg_sq=16, device_state=16, ticket=16)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return lib.pinn_adamw_group_step(ctypes.byref(d), one, one, None)
+    assert lib.pinn_adamw_group_step(None, one, one, None) == NULL
+    assert lib.pinn_adamw_group_step(ctypes.byref(PinnAdamWGroup()), None, one, None) == NULL
+    for kw in (dict(n_tensors=-1), dict(n_tensors=241), dict(n_chunks=-1), dict(dtype=3), dict(dtype=-1), dict(state_bits=16), dict(n_partials=-1), dict(master=16)):
+        assert group(**kw) == INVALID, kw
+    for kw in (dict(spans=None), dict(chunk_tensor=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(device_state=None), dict(ticket=None),
+               dict(state_bits=8), dict(n_partials=4)):
+        assert group(**kw) == NULL, kw
+    assert group(n_tensors=0) == 0 and group(n_chunks=0) == 0
+    d = PinnAdamWGroup(n_tensors=1, n_chunks=1, state_bits=32, spans=16, chunk_tensor=16, exp_avg=16, exp_avg_sq=16, device_state=16, ticket=16)
+    zero = (ctypes.c_uint64 * 1)(0)
+    assert lib.pinn_adamw_group_step(ctypes.byref(d), zero, one, None) == NULL
+    assert lib.pinn_adamw_group_step(ctypes.byref(d), zero, zero, None) == 0                    # no gradient: nothing to do
+
+    assert lib.pinn_adamw_moments(16, 16, 16, 16, 16, 16, 100, None) == INVALID
+    assert lib.pinn_adamw_moments(16, 16, 16, 16, 16, 16, -128, None) == INVALID
+    assert lib.pinn_adamw_moments(16, None, 16, 16, 16, 16, 128, None) == NULL
+    assert lib.pinn_adamw_moments(None, None, None, None, None, None, 0, None) == 0
+
+    assert lib.pinn_grad_norm_partials(-1) == INVALID and lib.pinn_grad_norm_partials(0) == 0
+    assert lib.pinn_grad_norm_partials(160) == 1024 and lib.pinn_grad_norm_partials(161) == 2048
+    count = ctypes.c_int32()
+    n2, f32 = (ctypes.c_int64 * 2)(100, 100), (ctypes.c_int32 * 2)(0, 0)
+
+    def sums(x=one, n=n2, dt=f32, k=2, part=16, room=4096):
+        return lib.pinn_grad_sumsq(x, n, dt, k, part, room, ctypes.byref(count), None)
+    assert sums(k=-1) == INVALID and sums(n=(ctypes.c_int64 * 2)(5, -1)) == INVALID and sums(dt=(ctypes.c_int32 * 2)(0, 7)) == INVALID
+    assert sums(x=None) == NULL and sums(part=None) == NULL and sums(x=(ctypes.c_uint64 * 2)(16, 0)) == NULL
+    assert sums(n=(ctypes.c_int64 * 2)(1, 1 << 62)) == LARGE and sums(room=1) == LARGE
+    assert lib.pinn_grad_sumsq(one, n2, f32, 2, 16, 4096, None, None) == NULL
+    assert lib.pinn_grad_norm(None, 1, 16, None) == NULL and lib.pinn_grad_norm(16, -1, 16, None) == INVALID
+
+    def clip(x=one, n=n2, k=2, part=16, m=1.0, out=16, np_=1):
+        return lib.pinn_grad_clip(x, n, f32, k, part, np_, m, out, None)
+    assert clip(m=-1.0) == INVALID and clip(m=float("nan")) == INVALID and clip(np_=-1) == INVALID
+    assert clip(part=None) == NULL and clip(out=None) == NULL
+    assert clip(x=(ctypes.c_uint64 * 2)(4096, 4096 + 396)) == OVERLAP and clip(x=(ctypes.c_uint64 * 2)(8192, 8192)) == OVERLAP
+    assert lib.pinn_error_string(OVERLAP) == b"two tensors share memory"
+
+
+def test_options_that_need_the_grouped_step():
+    from test_host_logic import feed, make_model
+    from pde_amd import scripts
+    g = np.load(os.path.join(GOLDEN, "burgers_9x20_xavier.npz"))
+    for kw in (dict(max_grad_norm=1.0), dict(adam_state_bits=8), dict(adam_impl="torch", max_grad_norm=1.0)):
+        m = make_model(g, scripts.burgers.PI.PhysicsInformedNN)
+        feed(m, g, "burgers")
+        for k, v in kw.items():
+            setattr(m, k, v)
+        with pytest.raises(ValueError, match="grouped"):
+            m.train(1, LBFGS_max_iter=0)
+    m = make_model(g, scripts.burgers.PI.PhysicsInformedNN)
+    feed(m, g, "burgers")
+    m.adam_impl = "grouped"
+    with pytest.raises(NativeError, match="no CPU fallback"):
+        m.train(1, LBFGS_max_iter=0)
