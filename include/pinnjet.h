@@ -261,7 +261,7 @@ int pinn_adam_step(float *theta, const float *grad, float *exp_avg, float *exp_a
  *   f = min(1, max_norm / (norm + 1e-6));  m = b1 m + (1 - b1) f g;  v = b2 v + (1 - b2) (f g)^2
  *   p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)
  * Moments, master weights and scales are flat device buffers in which every tensor starts at a multiple of
- * PINN_ADAMW_BLOCK elements (`offset` below); the elements behind a tensor's end are not written to (8 bits: they hold 0).
+ * PINN_ADAMW_BLOCK elements; the elements behind a tensor's end are not written to (8 bits: they hold 0).
  * 8-bit moments: one scale byte s per block, 2^(s - 127), 255 = the block holds a value that is not finite (it reads NaN
  * from then on); exp_avg: sign, 4 bits of exponent (bias 7), 3 of mantissa; exp_avg_sq: 5 bits of exponent (bias 15), 3 of mantissa.
  * They are rounded up or down by a sequence over steps and elements that is even on both sides; a positive v never becomes 0.
@@ -271,21 +271,24 @@ int pinn_adam_step(float *theta, const float *grad, float *exp_avg, float *exp_a
 #define PINN_BF16 1
 #define PINN_F16 2
 #define PINN_ADAMW_BLOCK 128         /* elements that share a scale */
-#define PINN_ADAMW_CHUNK 2048        /* elements per entry of chunk_tensor */
+#define PINN_ADAMW_CHUNK32 1024      /* elements a workgroup takes at a time, with float32 moments */
+#define PINN_ADAMW_CHUNK8 2048       /* the same with 8-bit moments */
 #define PINN_ADAMW_MAX_TENSORS 240   /* tensors per call: their addresses are launch arguments */
-#define PINN_ADAMW_GRID 2048         /* most workgroups of a step */
+#define PINN_ADAMW_TICKET_WORDS 2080 /* words of the ticket buffer */
 #define PINN_NORM_PARTIALS 1024      /* most partial sums per launch of pinn_grad_sumsq */
 
-typedef struct {
-    int64_t numel;
-    int64_t offset;                  /* first element in the flat buffers, a multiple of PINN_ADAMW_BLOCK */
-    int64_t first_chunk;             /* first entry in chunk_tensor */
-    int64_t row;                     /* row of device_state */
-} PinnTensorSpan;
+typedef struct {                     /* PINN_ADAMW_CHUNK32 or _CHUNK8 elements of one tensor, or the rest of it */
+    int64_t base;                    /* first element in the tensor, a multiple of the chunk */
+    int64_t place;                   /* the same element in the flat buffers: the tensor's start there, a multiple of PINN_ADAMW_BLOCK, + base */
+    int32_t count;                   /* 1 .. the chunk */
+    int32_t tensor;                  /* 0 .. n_tensors - 1: index in params, grads and rows */
+    int32_t row;                     /* rows[tensor] */
+    int32_t reserved;
+} PinnAdamWChunk;
 
 typedef struct {
-    const PinnTensorSpan *spans;     /* device, one per tensor of the call */
-    const uint16_t *chunk_tensor;    /* device: the tensor (0 .. n_tensors - 1) of each chunk, ceil(numel / PINN_ADAMW_CHUNK) per tensor, in order */
+    const PinnAdamWChunk *chunks;    /* device, in order: all chunks of the call's tensors */
+    const int32_t *rows;             /* device: each tensor's row of device_state */
     int64_t n_chunks;
     int32_t n_tensors;
     int32_t dtype;                   /* of parameters and gradients */
@@ -294,8 +297,8 @@ typedef struct {
     void *exp_avg, *exp_avg_sq;      /* float32, or codes */
     uint8_t *exp_avg_scale, *exp_avg_sq_scale;
     float *master;                   /* NULL: none; else the weights that are updated, the parameters are their rounded copy */
-    double *device_state;            /* rows of step, beta1^step, beta2^step; zeros to start */
-    uint32_t *ticket;                /* zero to start; every call leaves it zero */
+    double *device_state;            /* rows of step, beta1^step, beta2^step; 0, 1, 1 to start */
+    uint32_t *ticket;                /* PINN_ADAMW_TICKET_WORDS words, zero to start; every call leaves them zero */
     const double *partials;          /* from pinn_grad_sumsq, over the tensors that are clipped together */
     int32_t n_partials;              /* 0: no norm */
     int32_t reserved;

@@ -5,6 +5,7 @@ missing or no GPU is present, constructing a NativeEngine raises.
 import ctypes
 import os
 
+import numpy as np
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -27,12 +28,13 @@ class PinnDesc(ctypes.Structure):
     ]
 
 
-class PinnTensorSpan(ctypes.Structure):
-    _fields_ = [("numel", ctypes.c_int64), ("offset", ctypes.c_int64), ("first_chunk", ctypes.c_int64), ("row", ctypes.c_int64)]
+# PinnAdamWChunk
+ADAMW_CHUNK_DTYPE = np.dtype([("base", np.int64), ("place", np.int64), ("count", np.int32), ("tensor", np.int32), ("row", np.int32),
+                              ("reserved", np.int32)])
 
 
 class PinnAdamWGroup(ctypes.Structure):
-    _fields_ = ([(k, ctypes.c_void_p) for k in ("spans", "chunk_tensor")] + [("n_chunks", ctypes.c_int64)]
+    _fields_ = ([(k, ctypes.c_void_p) for k in ("chunks", "rows")] + [("n_chunks", ctypes.c_int64)]
                 + [(k, ctypes.c_int32) for k in ("n_tensors", "dtype", "state_bits", "skip_nonfinite")]
                 + [(k, ctypes.c_void_p) for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master",
                                                   "device_state", "ticket", "partials")]
@@ -42,7 +44,7 @@ class PinnAdamWGroup(ctypes.Structure):
 
 # include/pinnjet.h: dtype codes and the constants of the AdamW step over many tensors
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_TENSORS = 128, 2048, 240
+ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS = 128, 1024, 2048, 240, 2080
 ERR_OVERLAP = -7
 
 

@@ -5,7 +5,7 @@
 //   p <- (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Every element is read and written once (28 bytes for float32 throughout), so the step is bound by memory.  The tensors
-// are cut into chunks of kChunk elements; a table that the caller keeps on the device says which tensor a chunk lies in, so
+// are cut into chunks of 1024 or 2048 elements; a table that the caller keeps on the device says which tensor a chunk lies in, so
 // one launch covers up to kMaxTensors tensors of any sizes; their addresses travel in the launch's arguments, because
 // gradients move from step to step.  Moments and master weights are flat buffers in which each tensor starts at a multiple of kBlock.
 //
@@ -29,32 +29,57 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = PINN_ADAMW_BLOCK;        // elements that share a scale; also the layout's alignment
-constexpr int kChunk = PINN_ADAMW_CHUNK;        // elements a workgroup takes at a time
+constexpr int kChunk32 = PINN_ADAMW_CHUNK32, kChunk8 = PINN_ADAMW_CHUNK8;   // elements a workgroup takes at a time
 constexpr int kMaxTensors = PINN_ADAMW_MAX_TENSORS;
+// Bytes of LDS that a step's workgroups ask for and do not use: 6 or 5 of them fit on a CU instead of 8.  More streams of reads and writes
+// at once cost memory bandwidth.  float32 moments, 240M float32 weights (28 bytes each): 8 workgroups of 2048 elements 1186 us, 5 of them 1138,
+// 5 of 1024 elements 1099, 6 of 1024 elements 1082 (6.2 TB/s), 3 of 1024 elements 1394.  8-bit moments, 240M float32 weights (16 bytes): free 673 us, 5 workgroups 653.
+constexpr unsigned kPace32 = 27000, kPace8 = 32000;
 constexpr int kNormTensors = 160;
 constexpr int kNormChunk = 8192;
 constexpr int kMaxPartials = PINN_NORM_PARTIALS;
-static_assert(sizeof(PinnTensorSpan) == 32 && sizeof(PinnAdamWGroup) == 168, "the callers' layouts");
-static_assert(kChunk == 8 * kThreads && kChunk % kBlock == 0, "a thread takes 8 elements of a chunk");
+static_assert(sizeof(PinnAdamWChunk) == 32 && sizeof(PinnAdamWGroup) == 168, "the callers' layouts");
+static_assert(kChunk32 == 4 * kThreads && kChunk8 == 8 * kThreads && kChunk32 % kBlock == 0, "a thread takes 4 or 8 elements of a chunk");
 
-// N elements at any address that an element may have: the loads stay wide, the hardware takes them unaligned
+// N elements at any address that an element may have: the accesses stay wide, the hardware takes them unaligned.  Everything
+// here is touched once per step: the non-temporal forms keep it from displacing what is used again (240M float32 weights, step with
+// clipping, before the later changes: 1.60 ms plain, 1.53 ms with both; loads or stores alone 1.63, 1.60).
 template <class T, int N>
-__device__ inline void load(const T *p, T (&out)[N])
+using Vec = T __attribute__((ext_vector_type(N)));
+
+template <int N, class T>
+__device__ inline Vec<T, N> load(const T *p)
 {
     typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-    const V x = *(const V *)p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = x[i];
+    return __builtin_nontemporal_load((const V *)p);
 }
 
-template <class T, int N>
-__device__ inline void store(T *p, const T (&in)[N])
+template <int N, class T>
+__device__ inline void store(T *p, Vec<T, N> x)
 {
     typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-    V x;
+    __builtin_nontemporal_store((V)x, (V *)p);
+}
+
+// the first `have` of N elements and zeros behind them; FULL: all are there
+template <bool FULL, int N, class T>
+__device__ inline Vec<T, N> load_some(const T *p, int have)
+{
+    if (FULL || have >= N) return load<N>(p);
+    Vec<T, N> x = (T)0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = in[i];
-    *(V *)p = x;
+    for (int e = 0; e < N; ++e)
+        if (e < have) x[e] = p[e];
+    return x;
+}
+
+template <bool FULL, int N, class T>
+__device__ inline void store_some(T *p, Vec<T, N> x, int have)
+{
+    if (FULL || have >= N) return store<N>(p, x);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (e < have) p[e] = x[e];
 }
 
 // float32 rounded once to T.  The empty asm keeps the compiler from folding a float16 conversion into the fma before it
@@ -62,7 +87,7 @@ __device__ inline void store(T *p, const T (&in)[N])
 template <class T>
 __device__ inline T rounded(float x)
 {
-    if constexpr (sizeof(T) == 2) asm("" : "+v"(x));
+    if constexpr (__is_same(T, _Float16)) asm("" : "+v"(x));
     return (T)x;
 }
 
@@ -70,9 +95,10 @@ struct StepArgs {
     void *p[kMaxTensors];
     const void *g[kMaxTensors];                 // null: no gradient, the tensor is left alone
 };
+typedef const __attribute__((address_space(4))) PinnAdamWChunk ConstChunk;   // read-only while the kernel runs: scalar loads
 struct StepConst {
-    const PinnTensorSpan *span;
-    const uint16_t *chunk_tensor;
+    const PinnAdamWChunk *chunks;
+    const int32_t *rows;
     uint8_t *m, *v, *sm, *sv;                   // m, v: float32 or codes; sm, sv: scales
     float *master;
     double *state;                              // [tensor][3]: step, b1^t, b2^t
@@ -80,7 +106,7 @@ struct StepConst {
     const double *partials;
     float *norm_out;
     int64_t n_chunks;
-    int32_t n_tensors, n_partials, skip_nonfinite;
+    int32_t n_tensors, n_partials, skip_nonfinite, run;
     double max_norm, b1, b2, lr;
     float eps, decay;
 };
@@ -90,6 +116,7 @@ static_assert(sizeof(StepArgs) + sizeof(StepConst) <= 4096, "a launch's argument
 __device__ double sum_partials(const double *partials, int n)
 {
     __shared__ double part[kThreads / 64];
+    if (n == 1) return partials[0];
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += kThreads) s += partials[i];
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
@@ -113,15 +140,22 @@ struct Scalars {
     uint32_t t;
 };
 
+// v_rcp_f64 and v_sqrt_f64 are good to about 2^-25; one Newton step gives the reciprocal twice the digits.  A full division and
+// root are 60 instructions, which a workgroup of 2048 elements feels.
+__device__ inline double reciprocal(double x)
+{
+    const double r = __builtin_amdgcn_rcp(x);
+    return fma(r, fma(-x, r, 1.0), r);
+}
+
 __device__ inline Scalars scalars_of(const double *row, double b1, double b2, double lr)
 {
     Scalars s;
-    const double t0 = row[0];
-    s.p1 = (t0 == 0.0 ? 1.0 : row[1]) * b1;
-    s.p2 = (t0 == 0.0 ? 1.0 : row[2]) * b2;
-    s.t = (uint32_t)(int64_t)(t0 + 1.0);
-    s.step_size = (float)(lr / (1.0 - s.p1));
-    s.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - s.p2));
+    s.t = (uint32_t)(row[0] + 1.0);
+    s.p1 = row[1] * b1;
+    s.p2 = row[2] * b2;
+    s.step_size = (float)(lr * reciprocal(1.0 - s.p1));
+    s.inv_bc2_sqrt = (float)reciprocal(__builtin_amdgcn_sqrt(1.0 - s.p2));
     return s;
 }
 
@@ -139,47 +173,50 @@ __device__ inline void update32(float &p, float g, float &m, float &v, const Sca
     p = fmaf(-s.step_size, m / denom, p);
 }
 
-template <class T, bool MASTER>
-__device__ inline void chunk32(T *p, const T *g, float *m, float *v, float *master, int64_t left, const Scalars &s, const Hyper32 &h)
+// Where a chunk's data lie.
+template <class T>
+struct At {
+    T *p;
+    const T *g;                                 // null: no gradient, nothing to do
+    uint8_t *m, *v, *sm, *sv;
+    float *master;
+    uint32_t place;
+    int count;
+    const double *row;
+};
+
+template <bool FULL, bool MASTER, class T>
+__device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper32 &h)
 {
-    constexpr int N = 4, J = kChunk / (N * kThreads);
+    constexpr int N = 4;
+    float *am = (float *)at.m, *av = (float *)at.v;
+    const int i = (int)threadIdx.x * N, have = at.count - i;
+    if (!FULL && have <= 0) return;
+    const Vec<T, N> g = load_some<FULL, N>(at.g + i, have);
+    Vec<T, N> p;
+    Vec<float, N> w, m, v;
+    if constexpr (MASTER) w = load_some<FULL, N>(at.master + i, have);
+    else p = load_some<FULL, N>(at.p + i, have);
+    m = load_some<FULL, N>(am + i, have);
+    v = load_some<FULL, N>(av + i, have);
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int64_t i = (int64_t)(j * kThreads + threadIdx.x) * N;
-        if (i + N <= left) {
-            T pt[N], gt[N];
-            float pf[N], mf[N], vf[N];
-            load(g + i, gt);
-            if constexpr (MASTER) load(master + i, pf);
-            else load(p + i, pt);
-            load(m + i, mf);
-            load(v + i, vf);
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                if constexpr (!MASTER) pf[e] = (float)pt[e];
-                update32(pf[e], (float)gt[e], mf[e], vf[e], s, h);
-                pt[e] = rounded<T>(pf[e]);
-            }
-            store(p + i, pt);
-            if constexpr (MASTER) store(master + i, pf);
-            store(m + i, mf);
-            store(v + i, vf);
-        } else {
-            for (int64_t e = i; e < left; ++e) {
-                float pf = MASTER ? master[e] : (float)p[e], mf = m[e], vf = v[e];
-                update32(pf, (float)g[e], mf, vf, s, h);
-                p[e] = rounded<T>(pf);
-                if constexpr (MASTER) master[e] = pf;
-                m[e] = mf;
-                v[e] = vf;
-            }
-        }
+    for (int e = 0; e < N; ++e) {
+        float we = MASTER ? w[e] : (float)p[e], me = m[e], ve = v[e];
+        update32(we, (float)g[e], me, ve, s, h);
+        w[e] = we;
+        m[e] = me;
+        v[e] = ve;
+        p[e] = rounded<T>(we);
     }
+    store_some<FULL, N>(at.p + i, p, have);
+    if constexpr (MASTER) store_some<FULL, N>(at.master + i, w, have);
+    store_some<FULL, N>(am + i, m, have);
+    store_some<FULL, N>(av + i, v, have);
 }
 
 // ---- 8-bit moments ---------------------------------------------------------------------------------------------
 struct Format {
-    int shift;        // the smallest normal code's exponent against float64's (2^-1022): value * 2^-shift puts code bits on top of the upper word
+    int shift;        // the smallest normal code's exponent against float64's (2^-1022): value * 2^-shift puts the code on top of the upper word
     int shift32;      // the same against float32's 2^-126, for decoding
     int top;          // exponent of the largest code's magnitude, 1.75 * 2^top
     int most_scale;   // largest scale byte: the largest code stays finite in float32
@@ -210,166 +247,241 @@ __device__ inline int scale_of(uint32_t hi, const Format &f)
     return s < 0 ? 0 : s > f.most_scale ? f.most_scale : s;
 }
 
-__device__ inline uint32_t code_of(double x, int scale, uint32_t w, const Format &f)
+// x's magnitude as a code before it is held to the largest: 3 ldexp'd mantissa bits and what the remainder adds
+__device__ inline uint32_t code_of(double x, int exponent, uint32_t w)
 {
-    const uint32_t hi = (uint32_t)__double2hiint(ldexp(x, 127 - scale - f.shift)) & 0x7fffffffu;
-    const uint32_t c = (hi + (w >> 15 | 1u)) >> 17;
-    return c > f.most_code ? f.most_code : c;
+    const uint32_t hi = (uint32_t)__double2hiint(ldexp(fabs(x), exponent));
+    return (hi + (w >> 15 | 1u)) >> 17;
 }
 
 // the sequences that round: golden ratio, sqrt(2) over the elements; the two-dimensional analogue of the golden ratio over the steps
 constexpr uint32_t kPlaceM = 0x9E3779B9u, kStepM = 0xC13FA9A9u, kPlaceV = 0x6A09E667u, kStepV = 0x91E10DA5u;
 
 struct Hyper8 {
-    double b1, b2, omb1, omb2, factor;
+    double b1, b2, g1, g2;                      // g1 = (1 - b1) f, g2 = (1 - b2) f^2
     float eps, decay;
 };
 
-template <class T, bool MASTER>
-__device__ inline void chunk8(T *p, const T *g, uint8_t *m, uint8_t *v, uint8_t *sm, uint8_t *sv, float *master, int64_t place, int64_t left,
-                              const Scalars &s, const Hyper8 &h)
+// A lane's 8 elements of a block: two runs of 4, APART elements from each other.  16-bit weights without masters: one run of 8
+// (16 bytes).  With float32 among them the runs are half a block apart, so that 16 lanes read 256 bytes in a row and not every
+// other 16 (240M float32 weights: 652 us, with one run of 8 766).
+template <bool FULL, int APART, class T>
+__device__ inline Vec<T, 8> load_runs(const T *p, int have)
 {
-    constexpr int N = 8;
-    const int i = (int)threadIdx.x * N;         // a block is 16 lanes: a DPP row
-    if ((int64_t)(i & ~(kBlock - 1)) >= left) return;   // whole rows leave together
-    const int have = left - i >= N ? N : left - i <= 0 ? 0 : (int)(left - i);
-    T gt[N], pt[N];
-    float pf[N];
-    if (have == N) {
-        load(g + i, gt);
-        if constexpr (MASTER) load(master + i, pf);
-        else load(p + i, pt);
+    if constexpr (APART == 4) return load_some<FULL, 8>(p, have);
+    const Vec<T, 4> a = load_some<FULL, 4>(p, have), b = load_some<FULL, 4>(p + APART, have - APART);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <bool FULL, int APART, class T>
+__device__ inline void store_runs(T *p, Vec<T, 8> x, int have)
+{
+    if constexpr (APART == 4) return store_some<FULL, 8>(p, x, have);
+    store_some<FULL, 4>(p, __builtin_shufflevector(x, x, 0, 1, 2, 3), have);
+    store_some<FULL, 4>(p + APART, __builtin_shufflevector(x, x, 4, 5, 6, 7), have - APART);
+}
+
+template <bool FULL, bool MASTER, class T>
+__device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper8 &h)
+{
+    constexpr int N = 8, APART = sizeof(T) == 4 || MASTER ? kBlock / 2 : 4;
+    const int lane = (int)threadIdx.x & 15, blk = (int)threadIdx.x >> 4;    // a block is 16 lanes, a DPP row
+    const int i = blk * kBlock + lane * (APART == 4 ? 8 : 4), have = at.count - i;
+    if (!FULL && blk * kBlock >= at.count) return;     // rows behind the tensor's end leave together
+    Vec<uint32_t, 2> cm, cv;
+    if constexpr (APART == 4) {
+        cm = load<2>((const uint32_t *)(at.m + i));
+        cv = load<2>((const uint32_t *)(at.v + i));
     } else {
-        for (int e = 0; e < N; ++e) {
-            gt[e] = e < have ? g[i + e] : (T)0.0f;
-            if constexpr (MASTER) pf[e] = e < have ? master[i + e] : 0.0f;
-            else pt[e] = e < have ? p[i + e] : (T)0.0f;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            cm[r] = load<1>((const uint32_t *)(at.m + i + r * APART))[0];
+            cv[r] = load<1>((const uint32_t *)(at.v + i + r * APART))[0];
         }
     }
-    const uint2 cm = *(const uint2 *)(m + i), cv = *(const uint2 *)(v + i);
-    const int blk = i / kBlock;
-    const int s0m = sm[blk], s0v = sv[blk];
-    const double nan = __hiloint2double(0x7ff80000, 0);
-    const double um = s0m == 255 ? nan : h.b1 * pow2(s0m - 127 + kM.shift32);
-    const double uv = s0v == 255 ? nan : h.b2 * pow2(s0v - 127 + kV.shift32);
+    const int s0m = at.sm[blk], s0v = at.sv[blk];
+    const Vec<T, N> g = load_runs<FULL, APART>(at.g + i, have);
+    Vec<T, N> p;
+    Vec<float, N> w;
+    if constexpr (MASTER) w = load_runs<FULL, APART>(at.master + i, have);
+    else p = load_runs<FULL, APART>(at.p + i, have);
+    double um = h.b1 * pow2(s0m - 127), uv = h.b2 * pow2(s0v - 127 + kV.shift32);
+    if (s0m == 255) um = __hiloint2double(0x7ff80000, 0);
+    if (s0v == 255) uv = __hiloint2double(0x7ff80000, 0);
+    asm("" : "+v"(um), "+v"(uv));               // or the compiler makes the NaN a choice behind every product
     double md[N], vd[N];
     uint32_t hm = 0, hv = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        const uint32_t bm = ((e < 4 ? cm.x : cm.y) >> (8 * (e & 3))) & 255u, bv = ((e < 4 ? cv.x : cv.y) >> (8 * (e & 3))) & 255u;
-        const double gd = (double)(float)gt[e] * h.factor;
-        md[e] = fma((double)__uint_as_float((bm & 127u) << 20 | (bm & 128u) << 24), um, h.omb1 * gd);
-        vd[e] = fma((double)__uint_as_float(bv << 20), uv, h.omb2 * gd * gd);
-        const uint32_t am = (uint32_t)__double2hiint(md[e]) & 0x7fffffffu, av = (uint32_t)__double2hiint(vd[e]) & 0x7fffffffu;
+        // m's codes are the hardware's 8-bit floats (OCP E4M3; its NaN, 127, is never written)
+        const int pair = (int)cm[e / 4];
+        const float fm = (e & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(pair, true) : __builtin_amdgcn_cvt_pk_f32_fp8(pair, false))[e & 1];
+        const float fv = __uint_as_float((e & 3) == 3 ? cv[e / 4] >> 4 & 0x0ff00000u : cv[e / 4] << (20 - 8 * (e & 3)) & 0x0ff00000u);
+        const double gd = (double)(float)g[e];
+        md[e] = fma((double)fm, um, h.g1 * gd);
+        vd[e] = fma(h.g2 * gd, gd, (double)fv * uv);
+        const uint32_t am = (uint32_t)__double2hiint(md[e]) & 0x7fffffffu, av = (uint32_t)__double2hiint(vd[e]);
         hm = am > hm ? am : hm;
         hv = av > hv ? av : hv;
-        if constexpr (!MASTER) pf[e] = (float)pt[e];
-        const float denom = sqrtf((float)vd[e]) * s.inv_bc2_sqrt + h.eps;
-        pf[e] = fmaf(-s.step_size, (float)md[e] / denom, pf[e] * h.decay);
-        pt[e] = rounded<T>(pf[e]);
+        // v_sqrt_f64 is good to 2^-25 over all of float64, v_rcp_f32 to 2^-23: beside the weight's own rounding they do not show
+        const float denom = fmaf((float)__builtin_amdgcn_sqrt(vd[e]), s.inv_bc2_sqrt, h.eps);
+        const float we = fmaf(-s.step_size * (float)md[e], __builtin_amdgcn_rcpf(denom), (MASTER ? w[e] : (float)p[e]) * h.decay);
+        w[e] = we;
+        p[e] = rounded<T>(we);
     }
+    store_runs<FULL, APART>(at.p + i, p, have);
+    if constexpr (MASTER) store_runs<FULL, APART>(at.master + i, w, have);
     const int s1m = scale_of(row_max(hm), kM), s1v = scale_of(row_max(hv), kV);
-    const uint32_t at = (uint32_t)(place + i);
-    uint32_t wm = at * kPlaceM + s.t * kStepM, wv = at * kPlaceV + s.t * kStepV;
-    uint32_t om[2] = {0, 0}, ov[2] = {0, 0};
+    const int xm = 127 - s1m - kM.shift, xv = 127 - s1v - kV.shift;
+    const uint32_t place = at.place + i;
+    const uint32_t w0m = place * kPlaceM + s.t * kStepM, w0v = place * kPlaceV + s.t * kStepV;
+    Vec<uint32_t, 2> om = 0, ov = 0;
+    // behind the tensor's end gradients and codes are zero, and so are the codes that come out
 #pragma unroll
-    for (int e = 0; e < N; ++e, wm += kPlaceM, wv += kPlaceV) {
-        uint32_t a = code_of(md[e], s1m, wm, kM) | ((uint32_t)__double2hiint(md[e]) >> 24 & 128u);
-        uint32_t b = code_of(vd[e], s1v, wv, kV);
-        if (b == 0 && vd[e] > 0.0) b = 1;       // a v that vanished under a live m would divide it by eps alone
-        if (e >= have) a = b = 0;               // behind the tensor's end the codes stay zero
+    for (int e = 0; e < N; ++e) {
+        const uint32_t off = e < 4 ? e : APART + e - 4;
+        uint32_t a = code_of(md[e], xm, w0m + off * kPlaceM), b = code_of(vd[e], xv, w0v + off * kPlaceV);
+        a = a > kM.most_code ? kM.most_code : a;
+        a |= (uint32_t)__double2hiint(md[e]) >> 24 & 128u;
+        // 1 where v is not zero (written out: as a comparison it takes twice the instructions): a v that vanished under a live m would divide it by eps alone
+        uint32_t live;
+        asm("v_min_u32 %0, 1, %1" : "=v"(live) : "v"(__double2hiint(vd[e])));
+        asm("v_med3_u32 %0, %1, %2, %3" : "=v"(b) : "v"(b), "v"(live), "s"(kV.most_code));
         om[e / 4] |= a << (8 * (e & 3));
         ov[e / 4] |= b << (8 * (e & 3));
     }
-    if (s1m == 255) om[0] = om[1] = 0;
-    if (s1v == 255) ov[0] = ov[1] = 0;
-    *(uint2 *)(m + i) = make_uint2(om[0], om[1]);
-    *(uint2 *)(v + i) = make_uint2(ov[0], ov[1]);
-    if ((threadIdx.x & 15) == 0) {
-        sm[blk] = (uint8_t)s1m;
-        sv[blk] = (uint8_t)s1v;
-    }
-    if (have == N) {
-        store(p + i, pt);
-        if constexpr (MASTER) store(master + i, pf);
+    if (s1m == 255) om = 0;
+    if (s1v == 255) ov = 0;
+    if constexpr (APART == 4) {
+        store<2>((uint32_t *)(at.m + i), om);
+        store<2>((uint32_t *)(at.v + i), ov);
     } else {
-        for (int e = 0; e < have; ++e) {
-            p[i + e] = pt[e];
-            if constexpr (MASTER) master[i + e] = pf[e];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            store<1>((uint32_t *)(at.m + i + r * APART), Vec<uint32_t, 1>(om[r]));
+            store<1>((uint32_t *)(at.v + i + r * APART), Vec<uint32_t, 1>(ov[r]));
         }
+    }
+    if (lane == 0) {
+        at.sm[blk] = (uint8_t)s1m;
+        at.sv[blk] = (uint8_t)s1v;
     }
 }
 
+constexpr unsigned kTickets = 64, kTicketStride = 32;
+static_assert((kTickets + 1) * kTicketStride == PINN_ADAMW_TICKET_WORDS, "the callers' buffer");
+
+__device__ inline uint32_t draw(uint32_t *word)
+{
+    return __hip_atomic_fetch_add(word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ inline void put_back(uint32_t *word)
+{
+    __hip_atomic_store(word, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <class T>
+__device__ inline At<T> locate(const StepArgs &a, const StepConst &c, int64_t ch, int bits)
+{
+    ConstChunk &r = ((ConstChunk *)(uintptr_t)c.chunks)[ch];
+    const int64_t base = r.base, place = r.place;
+    const int k = r.tensor;
+    const int bytes = bits == 32 ? 4 : 1;
+    At<T> at;
+    at.g = (const T *)a.g[k] ? (const T *)a.g[k] + base : nullptr;
+    at.p = (T *)a.p[k] + base;
+    at.m = c.m + place * bytes;
+    at.v = c.v + place * bytes;
+    at.sm = c.sm + place / kBlock;
+    at.sv = c.sv + place / kBlock;
+    at.master = c.master + place;
+    at.place = (uint32_t)place;
+    at.count = r.count;
+    at.row = c.state + 3 * (int64_t)r.row;
+    return at;
+}
+
+// Workgroup b takes the chunks b * run .. b * run + run - 1.
 template <class T, bool MASTER, int BITS>
-__global__ __launch_bounds__(kThreads) void k_adamw_group(const StepArgs a, const StepConst c)
+__global__ __launch_bounds__(kThreads, BITS == 32 ? 6 : 5) void k_adamw_group(const StepArgs a, const StepConst c)
 {
     double factor = 1.0;
     if (c.n_partials) {
         const double norm = sqrt(sum_partials(c.partials, c.n_partials));
         if (c.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *c.norm_out = (float)norm;
-        if (c.skip_nonfinite && !(norm < __hiloint2double(0x7ff00000, 0))) return;   // in all workgroups alike: nothing is written, the ticket stays
+        if (c.skip_nonfinite && !(norm < __hiloint2double(0x7ff00000, 0))) return;   // in all workgroups alike: nothing is written, the tickets stay
         if (c.max_norm >= 0.0) factor = clip_factor(norm, c.max_norm);
     }
     Hyper32 h32;
     Hyper8 h8;
     if constexpr (BITS == 32) h32 = {(float)c.b2, (float)(1.0 - c.b1), (float)(1.0 - c.b2), c.eps, c.decay, (float)factor};
-    else h8 = {c.b1, c.b2, 1.0 - c.b1, 1.0 - c.b2, factor, c.eps, c.decay};
+    else h8 = {c.b1, c.b2, (1.0 - c.b1) * factor, (1.0 - c.b2) * factor * factor, c.eps, c.decay};
     Scalars s;
-    int last = -1;
-    for (int64_t ch = blockIdx.x; ch < c.n_chunks; ch += gridDim.x) {
-        const int k = c.chunk_tensor[ch];
-        const T *g = (const T *)a.g[k];
-        if (!g) continue;
-        const PinnTensorSpan sp = c.span[k];
-        const int64_t base = (ch - sp.first_chunk) * kChunk, left = sp.numel - base, at = sp.offset + base;
-        if (k != last) s = scalars_of(c.state + 3 * (int64_t)sp.row, c.b1, c.b2, c.lr);
-        last = k;
-        T *p = (T *)a.p[k];
-        if constexpr (BITS == 32)
-            chunk32<T, MASTER>(p + base, g + base, (float *)c.m + at, (float *)c.v + at, c.master + at, left, s, h32);
-        else
-            chunk8<T, MASTER>(p + base, g + base, c.m + at, c.v + at, c.sm + at / kBlock, c.sv + at / kBlock, c.master + at, at, left, s, h8);
+    const double *row = nullptr;
+    const int64_t first = (int64_t)blockIdx.x * c.run, end = first + c.run < c.n_chunks ? first + c.run : c.n_chunks;
+    for (int64_t ch = first; ch < end; ++ch) {
+        const At<T> at = locate<T>(a, c, ch, BITS);
+        if (!at.g) continue;
+        if (at.row != row) s = scalars_of(at.row, c.b1, c.b2, c.lr);
+        row = at.row;
+        if constexpr (BITS == 32) {
+            if (at.count == kChunk32) chunk<true, MASTER>(at, s, h32);
+            else chunk<false, MASTER>(at, s, h32);
+        } else {
+            if (at.count == kChunk8) chunk<true, MASTER>(at, s, h8);
+            else chunk<false, MASTER>(at, s, h8);
+        }
     }
-    // the workgroup that finishes last advances the counters: every other one has read them by then
-    __shared__ uint32_t done;
+    // The workgroup that finishes last advances the counters: every other one has used what it read of them by then.  Nothing
+    // else passes between workgroups, so the tickets need no fence (a device-wide one writes the caches back, once per workgroup).
+    // Atomics on one word take 11 ns each, one after the other (2048 of them 23 us, a third of a step of 5M weights): a
+    // workgroup draws from one of kTickets words on lines of their own, and the last of those draws from the first word.
+    __shared__ bool last_of_all;
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();
-        done = atomicAdd(c.ticket, 1u);
+        const unsigned groups = gridDim.x < kTickets ? gridDim.x : kTickets, j = blockIdx.x % kTickets;
+        uint32_t *mine = c.ticket + (1 + j) * kTicketStride;
+        last_of_all = false;
+        if (draw(mine) == (gridDim.x - j + kTickets - 1) / kTickets - 1) {
+            put_back(mine);
+            if (draw(c.ticket) == groups - 1) {
+                put_back(c.ticket);
+                last_of_all = true;
+            }
+        }
     }
     __syncthreads();
-    if (done != gridDim.x - 1) return;
+    if (!last_of_all) return;
     for (int k = threadIdx.x; k < c.n_tensors; k += kThreads)
         if (a.g[k]) {
-            double *row = c.state + 3 * (int64_t)c.span[k].row;
+            double *row = c.state + 3 * (int64_t)c.rows[k];
             const Scalars n = scalars_of(row, c.b1, c.b2, c.lr);
             row[0] += 1.0;
             row[1] = n.p1;
             row[2] = n.p2;
         }
-    if (threadIdx.x == 0) __hip_atomic_store(c.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // moments as float32: what the codes stand for
 __global__ __launch_bounds__(kThreads) void k_moments(const uint8_t *m, const uint8_t *v, const uint8_t *sm, const uint8_t *sv, float *mo,
                                                             float *vo, int64_t n)
 {
-    for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * kThreads * 4) {
-        const uint32_t cm = *(const uint32_t *)(m + i), cv = *(const uint32_t *)(v + i);
-        const int s0m = sm[i / kBlock], s0v = sv[i / kBlock];
-        float4 x, y;
-        float *xs = (float *)&x, *ys = (float *)&y;
+    const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
+    if (i >= n) return;
+    const uint32_t cm = load<1>((const uint32_t *)(m + i))[0], cv = load<1>((const uint32_t *)(v + i))[0];
+    const int s0m = sm[i / kBlock], s0v = sv[i / kBlock];
+    Vec<float, 4> x, y;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t a = cm >> (8 * e) & 255u, b = cv >> (8 * e) & 255u;
-            xs[e] = ldexpf(__uint_as_float((a & 127u) << 20 | (a & 128u) << 24), s0m - 127 + kM.shift32);
-            ys[e] = ldexpf(__uint_as_float(b << 20), s0v - 127 + kV.shift32);
-            if (s0m == 255) xs[e] = __uint_as_float(0x7fc00000u);
-            if (s0v == 255) ys[e] = __uint_as_float(0x7fc00000u);
-        }
-        *(float4 *)(mo + i) = x;
-        *(float4 *)(vo + i) = y;
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t a = cm >> (8 * e) & 255u, b = cv >> (8 * e) & 255u;
+        x[e] = ldexpf(__uint_as_float((a & 127u) << 20 | (a & 128u) << 24), s0m - 127 + kM.shift32);
+        y[e] = ldexpf(__uint_as_float(b << 20), s0v - 127 + kV.shift32);
+        if (s0m == 255) x[e] = __uint_as_float(0x7fc00000u);
+        if (s0v == 255) y[e] = __uint_as_float(0x7fc00000u);
     }
+    store<4>(mo + i, x);
+    store<4>(vo + i, y);
 }
 
 // ---- the global norm -------------------------------------------------------------------------------------------
@@ -394,21 +506,28 @@ __device__ inline int find_tensor(const NormArgs &a, int64_t ch)
     return lo;
 }
 
-template <class T>
-__device__ inline double chunk_sumsq(const T *x, int64_t left)
+template <class T, int N>
+__device__ inline void add_squares(double &s, Vec<T, N> x)
 {
-    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int e = 0; e < N; ++e) s = fma((double)(float)x[e], (double)(float)x[e], s);
+}
+
+template <class T>
+__device__ inline double chunk_sumsq(const T *x, int count)
+{
+    constexpr int N = 16 / sizeof(T), J = kNormChunk / (N * kThreads);
     double s = 0.0;
-    if (left >= kNormChunk) {
+    if (count == kNormChunk) {
+        Vec<T, N> t[J];                         // all loads of the chunk are under way before the first sum
 #pragma unroll
-        for (int j = 0; j < kNormChunk / (N * kThreads); ++j) {
-            T t[N];
-            load(x + (j * kThreads + threadIdx.x) * N, t);
+        for (int j = 0; j < J; ++j) t[j] = load<N>(x + (j * kThreads + threadIdx.x) * N);
 #pragma unroll
-            for (int e = 0; e < N; ++e) s = fma((double)(float)t[e], (double)(float)t[e], s);
-        }
+        for (int j = 0; j < J; ++j) add_squares<T, N>(s, t[j]);
     } else {
-        for (int64_t i = threadIdx.x; i < left; i += kThreads) s = fma((double)(float)x[i], (double)(float)x[i], s);
+        for (int i = threadIdx.x * N; i + N <= count; i += kThreads * N) add_squares<T, N>(s, load<N>(x + i));
+        const int i = count / N * N + (int)threadIdx.x;
+        if (i < count) s = fma((double)(float)x[i], (double)(float)x[i], s);
     }
     return s;
 }
@@ -420,9 +539,10 @@ __global__ __launch_bounds__(kThreads) void k_grad_sumsq(const NormArgs a, doubl
     for (int64_t ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
         const int k = find_tensor(a, ch);
         const int64_t base = (ch - a.first_chunk[k]) * kNormChunk, left = a.numel[k] - base;
-        if (a.dtype[k] == PINN_F32) s += chunk_sumsq((const float *)a.x[k] + base, left);
-        else if (a.dtype[k] == PINN_BF16) s += chunk_sumsq((const __bf16 *)a.x[k] + base, left);
-        else s += chunk_sumsq((const _Float16 *)a.x[k] + base, left);
+        const int count = left < kNormChunk ? (int)left : kNormChunk;
+        if (a.dtype[k] == PINN_F32) s += chunk_sumsq((const float *)a.x[k] + base, count);
+        else if (a.dtype[k] == PINN_BF16) s += chunk_sumsq((const __bf16 *)a.x[k] + base, count);
+        else s += chunk_sumsq((const _Float16 *)a.x[k] + base, count);
     }
     __shared__ double part[kThreads / 64];
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
@@ -435,6 +555,12 @@ __global__ __launch_bounds__(kThreads) void k_grad_sumsq(const NormArgs a, doubl
     }
 }
 
+__global__ __launch_bounds__(kThreads) void k_fold(double *partials, int n)
+{
+    const double s = sum_partials(partials, n);     // read by all before the barrier in there
+    if (threadIdx.x == 0) partials[0] = s;
+}
+
 __global__ __launch_bounds__(kThreads) void k_norm_of(const double *partials, int n, float *norm)
 {
     const double s = sum_partials(partials, n);
@@ -442,21 +568,18 @@ __global__ __launch_bounds__(kThreads) void k_norm_of(const double *partials, in
 }
 
 template <class T>
-__device__ inline void chunk_scale(T *x, int64_t left, float f)
+__device__ inline void chunk_scale(T *x, int count, float f)
 {
     constexpr int N = 16 / sizeof(T);
-    if (left >= kNormChunk) {
+#pragma unroll 4
+    for (int i = threadIdx.x * N; i + N <= count; i += kThreads * N) {
+        Vec<T, N> t = load<N>(x + i);
 #pragma unroll
-        for (int j = 0; j < kNormChunk / (N * kThreads); ++j) {
-            T t[N], *at = x + (j * kThreads + threadIdx.x) * N;
-            load(at, t);
-#pragma unroll
-            for (int e = 0; e < N; ++e) t[e] = (T)((float)t[e] * f);
-            store(at, t);
-        }
-    } else {
-        for (int64_t i = threadIdx.x; i < left; i += kThreads) x[i] = (T)((float)x[i] * f);
+        for (int e = 0; e < N; ++e) t[e] = (T)((float)t[e] * f);
+        store<N>(x + i, t);
     }
+    const int i = count / N * N + (int)threadIdx.x;
+    if (i < count) x[i] = (T)((float)x[i] * f);
 }
 
 __global__ __launch_bounds__(kThreads) void k_grad_clip(const NormArgs a, const double *partials, int n_partials, double max_norm, float *norm_out)
@@ -469,9 +592,10 @@ __global__ __launch_bounds__(kThreads) void k_grad_clip(const NormArgs a, const 
     for (int64_t ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
         const int k = find_tensor(a, ch);
         const int64_t base = (ch - a.first_chunk[k]) * kNormChunk, left = a.numel[k] - base;
-        if (a.dtype[k] == PINN_F32) chunk_scale((float *)a.x[k] + base, left, f);
-        else if (a.dtype[k] == PINN_BF16) chunk_scale((__bf16 *)a.x[k] + base, left, f);
-        else chunk_scale((_Float16 *)a.x[k] + base, left, f);
+        const int count = left < kNormChunk ? (int)left : kNormChunk;
+        if (a.dtype[k] == PINN_F32) chunk_scale((float *)a.x[k] + base, count, f);
+        else if (a.dtype[k] == PINN_BF16) chunk_scale((__bf16 *)a.x[k] + base, count, f);
+        else chunk_scale((_Float16 *)a.x[k] + base, count, f);
     }
 }
 
@@ -481,10 +605,17 @@ bool valid_dtype(int32_t d) { return d == PINN_F32 || d == PINN_BF16 || d == PIN
 int launch_error() { return hipGetLastError() == hipSuccess ? PINN_OK : PINN_ERR_HIP; }
 
 template <class T, bool MASTER>
-void launch_step(const StepArgs &a, const StepConst &c, int bits, unsigned grid, hipStream_t st)
+void launch_step(const StepArgs &a, StepConst c, int bits, hipStream_t st)
 {
-    if (bits == 32) hipLaunchKernelGGL((k_adamw_group<T, MASTER, 32>), dim3(grid), dim3(kThreads), 0, st, a, c);
-    else hipLaunchKernelGGL((k_adamw_group<T, MASTER, 8>), dim3(grid), dim3(kThreads), 0, st, a, c);
+    // 10 bytes an element (8-bit moments, 16-bit weights without masters) leave so little to wait for that the instructions count: such
+    // workgroups take 4 chunks each, which spreads the scalars of a step over more elements, and are not held back.  240M bfloat16
+    // weights: 1 chunk 518 us, 2 451, 4 432, 8 446; held to 5 workgroups 560.  All others are bound by memory and go fastest when workgroups
+    // come and go in the order of the addresses: 240M float32 weights, 8-bit moments: 1 chunk 773 us, 2 854, 4 957.
+    const bool lean = bits == 8 && sizeof(T) == 2 && !MASTER;
+    c.run = lean ? 4 : 1;
+    const unsigned grid = (unsigned)((c.n_chunks + c.run - 1) / c.run), pace = lean ? 0 : bits == 32 ? kPace32 : kPace8;
+    if (bits == 32) hipLaunchKernelGGL((k_adamw_group<T, MASTER, 32>), dim3(grid), dim3(kThreads), pace, st, a, c);
+    else hipLaunchKernelGGL((k_adamw_group<T, MASTER, 8>), dim3(grid), dim3(kThreads), pace, st, a, c);
 }
 
 // the tables of one launch after another over a list of tensors, and how many partial sums each writes
@@ -564,6 +695,12 @@ extern "C" int pinn_grad_sumsq(const void *const *grads, const int64_t *numel, c
         hipLaunchKernelGGL(k_grad_sumsq, dim3(plan.grid), dim3(kThreads), 0, (hipStream_t)stream, a, partials);
         *n_partials = plan.partials;
     }
+    // Whoever takes the partial sums adds them up in each of its workgroups: up to kThreads of them that is one load a thread, beyond it a
+    // launch of its own (3 us) is less than what thousands of workgroups spend on it.
+    if (*n_partials > kThreads) {
+        hipLaunchKernelGGL(k_fold, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, partials, *n_partials);
+        *n_partials = 1;
+    }
     return launch_error();
 }
 
@@ -599,8 +736,9 @@ extern "C" int pinn_adamw_group_step(const PinnAdamWGroup *d, void *const *param
     if (d->n_tensors < 0 || d->n_tensors > kMaxTensors || d->n_chunks < 0 || !valid_dtype(d->dtype) ||
         (d->state_bits != 32 && d->state_bits != 8) || d->n_partials < 0 || (d->master && d->dtype == PINN_F32))
         return PINN_ERR_INVALID_DESC;
+    if (d->n_chunks > INT32_MAX) return PINN_ERR_TOO_LARGE;
     if (d->n_tensors == 0 || d->n_chunks == 0) return PINN_OK;
-    if (!d->spans || !d->chunk_tensor || !d->exp_avg || !d->exp_avg_sq || !d->device_state || !d->ticket) return PINN_ERR_NULL;
+    if (!d->chunks || !d->rows || !d->exp_avg || !d->exp_avg_sq || !d->device_state || !d->ticket) return PINN_ERR_NULL;
     if (d->state_bits == 8 && (!d->exp_avg_scale || !d->exp_avg_sq_scale)) return PINN_ERR_NULL;
     if (d->n_partials && !d->partials) return PINN_ERR_NULL;
     StepArgs a;
@@ -613,8 +751,8 @@ extern "C" int pinn_adamw_group_step(const PinnAdamWGroup *d, void *const *param
     }
     if (!any) return PINN_OK;
     StepConst c;
-    c.span = d->spans;
-    c.chunk_tensor = d->chunk_tensor;
+    c.chunks = d->chunks;
+    c.rows = d->rows;
     c.m = (uint8_t *)d->exp_avg;
     c.v = (uint8_t *)d->exp_avg_sq;
     c.sm = d->exp_avg_scale;
@@ -634,15 +772,14 @@ extern "C" int pinn_adamw_group_step(const PinnAdamWGroup *d, void *const *param
     c.lr = d->lr;
     c.eps = (float)d->eps;
     c.decay = (float)(1.0 - d->lr * d->weight_decay);
-    const unsigned grid = (unsigned)(d->n_chunks < PINN_ADAMW_GRID ? d->n_chunks : PINN_ADAMW_GRID);
     const hipStream_t st = (hipStream_t)stream;
-    if (d->dtype == PINN_F32) launch_step<float, false>(a, c, d->state_bits, grid, st);
+    if (d->dtype == PINN_F32) launch_step<float, false>(a, c, d->state_bits, st);
     else if (d->dtype == PINN_BF16) {
-        if (d->master) launch_step<__bf16, true>(a, c, d->state_bits, grid, st);
-        else launch_step<__bf16, false>(a, c, d->state_bits, grid, st);
+        if (d->master) launch_step<__bf16, true>(a, c, d->state_bits, st);
+        else launch_step<__bf16, false>(a, c, d->state_bits, st);
     } else {
-        if (d->master) launch_step<_Float16, true>(a, c, d->state_bits, grid, st);
-        else launch_step<_Float16, false>(a, c, d->state_bits, grid, st);
+        if (d->master) launch_step<_Float16, true>(a, c, d->state_bits, st);
+        else launch_step<_Float16, false>(a, c, d->state_bits, st);
     }
     return launch_error();
 }
@@ -654,7 +791,8 @@ extern "C" int pinn_adamw_moments(const uint8_t *exp_avg, const uint8_t *exp_avg
     if (n == 0) return PINN_OK;
     if (!exp_avg || !exp_avg_sq || !exp_avg_scale || !exp_avg_sq_scale || !exp_avg_out || !exp_avg_sq_out) return PINN_ERR_NULL;
     const int64_t groups = (n / 4 + kThreads - 1) / kThreads;
-    hipLaunchKernelGGL(k_moments, dim3((unsigned)(groups < 8192 ? groups : 8192)), dim3(kThreads), 0, (hipStream_t)stream, exp_avg,
+    if (groups > INT32_MAX) return PINN_ERR_TOO_LARGE;
+    hipLaunchKernelGGL(k_moments, dim3((unsigned)groups), dim3(kThreads), 0, (hipStream_t)stream, exp_avg,
                        exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, exp_avg_out, exp_avg_sq_out, n);
     return launch_error();
 }

@@ -16,7 +16,7 @@ import ctypes
 import numpy as np
 import torch
 
-from ._native import (ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_TENSORS, DTYPE_CODES, ERR_OVERLAP, NativeError, PinnAdamWGroup, _check, _cur_stream,
+from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, DTYPE_CODES, ERR_OVERLAP, NativeError, PinnAdamWGroup, _check, _cur_stream,
                       _on, load_library)
 
 
@@ -326,8 +326,9 @@ class GroupedAdamW(torch.optim.Optimizer):
         if master_weights and any(p.dtype != torch.float32 for p in self._params):
             self.master = torch.zeros(at, dtype=torch.float32, device=dev)
             self.sync_master()
-        self.device_state = torch.zeros((len(self._params), 3), dtype=torch.float64, device=dev)   # step, beta1^step, beta2^step
-        self._ticket = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.device_state = torch.ones((len(self._params), 3), dtype=torch.float64, device=dev)    # step, beta1^step, beta2^step
+        self.device_state[:, 0] = 0.0
+        self._ticket = torch.zeros(ADAMW_TICKET_WORDS, dtype=torch.int32, device=dev)
         self._norm = torch.zeros((), dtype=torch.float32, device=dev)
         self._launches, first = [], 0
         for grp in self.param_groups:
@@ -339,17 +340,18 @@ class GroupedAdamW(torch.optim.Optimizer):
                     self._launches.append(self._launch(grp, dt, mine[a:a + ADAMW_MAX_TENSORS]))
 
     def _launch(self, grp, dtype, rows):
-        spans, chunks, at = [], [], 0
+        parts, chunk = [], ADAMW_CHUNK32 if self.state_bits == 32 else ADAMW_CHUNK8
         for k, i in enumerate(rows):
-            n = self._params[i].numel()
-            count = -(-n // ADAMW_CHUNK)
-            spans.append((n, self.offsets[i], at, i))
-            chunks.append(np.full(count, k, dtype=np.uint16))
-            at += count
-        spans = torch.from_numpy(np.array(spans, dtype=np.int64)).to(self.device)
-        chunks = torch.from_numpy(np.concatenate(chunks).view(np.int16)).to(self.device)
+            base = np.arange(0, self._params[i].numel(), chunk, dtype=np.int64)
+            part = np.zeros(len(base), dtype=ADAMW_CHUNK_DTYPE)
+            part["base"], part["place"], part["tensor"], part["row"] = base, self.offsets[i] + base, k, i
+            part["count"] = np.minimum(self._params[i].numel() - base, chunk)
+            parts.append(part)
+        parts = np.concatenate(parts)
+        chunks = torch.from_numpy(parts.view(np.uint8)).to(self.device)
+        where = torch.tensor(rows, dtype=torch.int32, device=self.device)
         d = PinnAdamWGroup()
-        d.spans, d.chunk_tensor, d.n_chunks, d.n_tensors = spans.data_ptr(), chunks.data_ptr(), at, len(rows)
+        d.chunks, d.rows, d.n_chunks, d.n_tensors = chunks.data_ptr(), where.data_ptr(), len(parts), len(rows)
         d.dtype, d.state_bits, d.skip_nonfinite = DTYPE_CODES[dtype], self.state_bits, int(self.skip_nonfinite)
         d.exp_avg, d.exp_avg_sq, d.device_state, d.ticket = (t.data_ptr() for t in (self.exp_avg, self.exp_avg_sq, self.device_state, self._ticket))
         if self.state_bits == 8:
@@ -357,7 +359,7 @@ class GroupedAdamW(torch.optim.Optimizer):
         if self.master is not None and dtype != torch.float32:
             d.master = self.master.data_ptr()
         d.max_norm = -1.0 if self.max_norm is None else self.max_norm
-        return dict(grp=grp, desc=d, rows=rows, p=(ctypes.c_uint64 * len(rows))(), g=(ctypes.c_uint64 * len(rows))(), tables=(spans, chunks))
+        return dict(grp=grp, desc=d, rows=rows, p=(ctypes.c_uint64 * len(rows))(), g=(ctypes.c_uint64 * len(rows))(), tables=(chunks, where))
 
     @torch.no_grad()
     def sync_master(self):

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import adamw_formulas as F
-from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK, ADAMW_MAX_TENSORS, NativeError, PinnAdamWGroup, PinnTensorSpan, load_library
+from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, NativeError, PinnAdamWGroup, load_library
 from pde_amd.optim import GroupedAdamW, clip_grad_norm_, grad_norm
 from conftest import GOLDEN, ROOT
 
@@ -78,14 +78,15 @@ def test_refusals_without_a_gpu():
 def test_c_entries_refuse_without_a_gpu():
     lib = load_library()
     header = open(os.path.join(ROOT, "include", "pinnjet.h")).read()
-    for name, value in (("PINN_ADAMW_BLOCK", ADAMW_BLOCK), ("PINN_ADAMW_CHUNK", ADAMW_CHUNK), ("PINN_ADAMW_MAX_TENSORS", ADAMW_MAX_TENSORS)):
+    for name, value in (("PINN_ADAMW_BLOCK", ADAMW_BLOCK), ("PINN_ADAMW_CHUNK32", ADAMW_CHUNK32), ("PINN_ADAMW_CHUNK8", ADAMW_CHUNK8), ("PINN_ADAMW_MAX_TENSORS", ADAMW_MAX_TENSORS),
+                        ("PINN_ADAMW_TICKET_WORDS", ADAMW_TICKET_WORDS)):
         assert "#define %s %d " % (name, value) in header
-    assert ctypes.sizeof(PinnTensorSpan) == 32 and ctypes.sizeof(PinnAdamWGroup) == 168
+    assert ADAMW_CHUNK_DTYPE.itemsize == 32 and ctypes.sizeof(PinnAdamWGroup) == 168
     one = (ctypes.c_uint64 * 2)(4096, 8192)
     INVALID, NULL, LARGE, OVERLAP = -1, -4, -6, -7
 
     def group(**kw):
-        d = PinnAdamWGroup(n_tensors=2, n_chunks=2, dtype=0, state_bits=32, spans=16, chunk_tensor=16, exp_avg=16, exp_avg_sq=16, device_state=16, ticket=16)
+        d = PinnAdamWGroup(n_tensors=2, n_chunks=2, dtype=0, state_bits=32, chunks=16, rows=16, exp_avg=16, exp_avg_sq=16, device_state=16, ticket=16)
         for k, v in kw.items():
             setattr(d, k, v)
         return lib.pinn_adamw_group_step(ctypes.byref(d), one, one, None)
@@ -93,11 +94,13 @@ def test_c_entries_refuse_without_a_gpu():
     assert lib.pinn_adamw_group_step(ctypes.byref(PinnAdamWGroup()), None, one, None) == NULL
     for kw in (dict(n_tensors=-1), dict(n_tensors=241), dict(n_chunks=-1), dict(dtype=3), dict(dtype=-1), dict(state_bits=16), dict(n_partials=-1), dict(master=16)):
         assert group(**kw) == INVALID, kw
-    for kw in (dict(spans=None), dict(chunk_tensor=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(device_state=None), dict(ticket=None),
+    for kw in (dict(chunks=None), dict(rows=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(device_state=None), dict(ticket=None),
                dict(state_bits=8), dict(n_partials=4)):
         assert group(**kw) == NULL, kw
+    assert group(n_chunks=1 << 40) == LARGE
+    assert lib.pinn_adamw_moments(16, 16, 16, 16, 16, 16, 1 << 50, None) == LARGE
     assert group(n_tensors=0) == 0 and group(n_chunks=0) == 0
-    d = PinnAdamWGroup(n_tensors=1, n_chunks=1, state_bits=32, spans=16, chunk_tensor=16, exp_avg=16, exp_avg_sq=16, device_state=16, ticket=16)
+    d = PinnAdamWGroup(n_tensors=1, n_chunks=1, state_bits=32, chunks=16, rows=16, exp_avg=16, exp_avg_sq=16, device_state=16, ticket=16)
     zero = (ctypes.c_uint64 * 1)(0)
     assert lib.pinn_adamw_group_step(ctypes.byref(d), zero, one, None) == NULL
     assert lib.pinn_adamw_group_step(ctypes.byref(d), zero, zero, None) == 0                    # no gradient: nothing to do
