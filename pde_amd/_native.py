@@ -118,6 +118,16 @@ def load_library():
     return lib
 
 
+def load_tensorlist():
+    """The in-tree extension module that reads lists of tensors (csrc/tensorlist.cpp); raises if it was not built."""
+    try:
+        from . import _tensorlist
+    except ImportError as ex:
+        raise NativeError("pde_amd/_tensorlist.so is missing or was built for another torch (%s): build it with "
+                          "`python -c 'import __graft_entry__ as g; g.build()'`" % ex) from ex
+    return _tensorlist
+
+
 def _check(rc, what):
     if rc != 0:
         msg = load_library().pinn_error_string(rc).decode()

@@ -1,0 +1,202 @@
+// Host side of the operators over many tensors: reads addresses, lengths and types of a list of torch tensors into the host arrays
+// that include/pinnjet.h's entry points take, and checks them on the way.  From Python the same takes 0.6 us a tensor, which for the
+// 240 tensors of 24 nets is five times the step itself; here it is 0.02.
+//
+// A Python extension module without GPU code; it knows nothing of a device beyond comparing tensors' devices.
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <exception>
+#include <stdint.h>
+
+namespace {
+
+int code_of(const at::Tensor &t)                // PINN_F32, PINN_BF16, PINN_F16; -1: none of them
+{
+    switch (t.scalar_type()) {
+    case at::kFloat: return 0;
+    case at::kBFloat16: return 1;
+    case at::kHalf: return 2;
+    default: return -1;
+    }
+}
+
+bool tensor_at(PyObject *list, Py_ssize_t i, const char *what)
+{
+    if (THPVariable_Check(PyList_GET_ITEM(list, i))) return true;
+    PyErr_Format(PyExc_TypeError, "%s %zd is a %s, a tensor is needed", what, i, Py_TYPE(PyList_GET_ITEM(list, i))->tp_name);
+    return false;
+}
+
+bool plain(const at::Tensor &t) { return t.layout() == at::kStrided && !t.is_neg() && !t.is_conj(); }
+
+// same order in memory: strides may differ where a dimension has one element
+bool same_order(const at::Tensor &a, const at::Tensor &b)
+{
+    if (a.is_contiguous() && b.is_contiguous()) return true;
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+    return true;
+}
+
+// no gaps and no overlaps
+bool dense(const at::Tensor &t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
+
+template <class F>
+PyObject *guarded(F f)
+{
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
+    }
+    return nullptr;
+}
+
+// gather(params, numel, dtype, p, g, count) -> (gradients found, [indices whose gradient lies in another order than its parameter])
+// numel, dtype: int64 and int32 arrays, what the plan was made for; p, g: uint64 arrays that take the addresses (g: 0 without a gradient);
+// count: int64 array, the gradient's length or 0.  Arrays are given by their address.
+PyObject *gather(PyObject *, PyObject *args)
+{
+    PyObject *params;
+    unsigned long long a_numel, a_dtype, a_p, a_g, a_count;
+    if (!PyArg_ParseTuple(args, "O!KKKKK", &PyList_Type, &params, &a_numel, &a_dtype, &a_p, &a_g, &a_count)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const int64_t *numel = (const int64_t *)(uintptr_t)a_numel;
+        const int32_t *dtype = (const int32_t *)(uintptr_t)a_dtype;
+        uint64_t *p_out = (uint64_t *)(uintptr_t)a_p, *g_out = (uint64_t *)(uintptr_t)a_g;
+        int64_t *count = (int64_t *)(uintptr_t)a_count;
+        const Py_ssize_t n = PyList_GET_SIZE(params);
+        PyObject *other = PyList_New(0);
+        if (!other) return nullptr;
+        Py_ssize_t given = 0;
+        c10::Device device(c10::DeviceType::CPU);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            if (!tensor_at(params, i, "parameter")) { Py_DECREF(other); return nullptr; }
+            const at::Tensor &p = THPVariable_Unpack(PyList_GET_ITEM(params, i));
+            if (i == 0) device = p.device();
+            if (!plain(p) || code_of(p) != dtype[i] || p.numel() != numel[i] || p.device() != device || !dense(p)) {
+                PyErr_Format(PyExc_ValueError, "parameter %zd is not what it was when the optimizer was made (type, size, device or layout)", i);
+                Py_DECREF(other);
+                return nullptr;
+            }
+            p_out[i] = (uint64_t)(uintptr_t)p.data_ptr();
+            g_out[i] = 0;
+            count[i] = 0;
+            const at::Tensor &g = p.grad();
+            if (!g.defined()) continue;
+            if (!plain(g) || g.scalar_type() != p.scalar_type() || g.device() != device || !g.sizes().equals(p.sizes())) {
+                PyErr_Format(PyExc_ValueError, "the gradient of parameter %zd is not a dense tensor of its parameter's type, shape and device", i);
+                Py_DECREF(other);
+                return nullptr;
+            }
+            if (numel[i] == 0) continue;
+            ++given;
+            count[i] = numel[i];
+            if (same_order(p, g)) {
+                g_out[i] = (uint64_t)(uintptr_t)g.data_ptr();
+            } else {
+                PyObject *k = PyLong_FromSsize_t(i);
+                const bool bad = !k || PyList_Append(other, k) != 0;
+                Py_XDECREF(k);
+                if (bad) { Py_DECREF(other); return nullptr; }
+            }
+        }
+        return Py_BuildValue("(nN)", given, other);
+    });
+}
+
+// describe(tensors, x, numel, dtype) -> [indices that are neither contiguous nor another order of the same memory]
+PyObject *describe(PyObject *, PyObject *args)
+{
+    PyObject *list;
+    unsigned long long a_x, a_numel, a_dtype;
+    if (!PyArg_ParseTuple(args, "O!KKK", &PyList_Type, &list, &a_x, &a_numel, &a_dtype)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        uint64_t *x = (uint64_t *)(uintptr_t)a_x;
+        int64_t *numel = (int64_t *)(uintptr_t)a_numel;
+        int32_t *dtype = (int32_t *)(uintptr_t)a_dtype;
+        const Py_ssize_t n = PyList_GET_SIZE(list);
+        PyObject *other = PyList_New(0);
+        if (!other) return nullptr;
+        c10::Device device(c10::DeviceType::CPU);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            if (!tensor_at(list, i, "tensor")) { Py_DECREF(other); return nullptr; }
+            const at::Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+            if (i == 0) device = t.device();
+            if (!plain(t) || code_of(t) < 0 || t.device() != device) {
+                PyErr_Format(PyExc_ValueError, "tensor %zd: dense float32, bfloat16 or float16 tensors on one device are needed, got %s on %s (the first is on %s)", i,
+                             !plain(t) ? "another layout" : c10::toString(t.scalar_type()), t.device().str().c_str(), device.str().c_str());
+                Py_DECREF(other);
+                return nullptr;
+            }
+            x[i] = (uint64_t)(uintptr_t)t.data_ptr();
+            numel[i] = t.numel();
+            dtype[i] = code_of(t);
+            if (!dense(t)) {
+                PyObject *k = PyLong_FromSsize_t(i);
+                const bool bad = !k || PyList_Append(other, k) != 0;
+                Py_XDECREF(k);
+                if (bad) { Py_DECREF(other); return nullptr; }
+            }
+        }
+        return other;
+    });
+}
+
+// grads(params) -> [gradient] of those that have one
+PyObject *grads(PyObject *, PyObject *list)
+{
+    if (!PyList_Check(list)) {
+        PyErr_SetString(PyExc_TypeError, "a list is needed");
+        return nullptr;
+    }
+    return guarded([&]() -> PyObject * {
+        PyObject *out = PyList_New(0);
+        if (!out) return nullptr;
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+            if (!tensor_at(list, i, "parameter")) { Py_DECREF(out); return nullptr; }
+            const at::Tensor &g = THPVariable_Unpack(PyList_GET_ITEM(list, i)).grad();
+            if (!g.defined()) continue;
+            PyObject *o = THPVariable_Wrap(g);
+            const bool bad = !o || PyList_Append(out, o) != 0;
+            Py_XDECREF(o);
+            if (bad) { Py_DECREF(out); return nullptr; }
+        }
+        return out;
+    });
+}
+
+// written(tensors, which): the tensors (those with which[i] != 0, an int64 array; 0: all) were written to in place
+PyObject *written(PyObject *, PyObject *args)
+{
+    PyObject *list;
+    unsigned long long a_which;
+    if (!PyArg_ParseTuple(args, "O!K", &PyList_Type, &list, &a_which)) return nullptr;
+    return guarded([&]() -> PyObject * {
+        const int64_t *which = (const int64_t *)(uintptr_t)a_which;
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+            if (which && !which[i]) continue;
+            if (!tensor_at(list, i, "tensor")) return nullptr;
+            const at::Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        }
+        Py_RETURN_NONE;
+    });
+}
+
+PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, nullptr},
+                         {"describe", describe, METH_VARARGS, nullptr},
+                         {"grads", grads, METH_O, nullptr},
+                         {"written", written, METH_VARARGS, nullptr},
+                         {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__tensorlist() { return PyModule_Create(&module); }

@@ -16,8 +16,8 @@ import ctypes
 import numpy as np
 import torch
 
-from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, DTYPE_CODES, ERR_OVERLAP, NativeError, PinnAdamWGroup, _check, _cur_stream,
-                      _on, load_library)
+from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, DTYPE_CODES, ERR_OVERLAP, NativeError, PinnAdamWGroup, _check, _cur_stream, _on, load_library,
+                      load_tensorlist)
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -142,48 +142,35 @@ def _flat(t):
     return t.as_strided((t.numel(),), (1,), t.storage_offset())
 
 
-class _GradList:
-    """Gradients as the C interface takes them: host arrays of addresses, lengths and types."""
+class _TensorList:
+    """Tensors as the C interface takes them: host arrays of addresses, lengths and types.  `back`: (tensor, copy) of those whose
+    memory has gaps or overlaps, the copy is what the arrays name."""
 
-    def __init__(self, grads, device, writable):
-        n = len(grads)
-        self.n, self.device, self.back, keep = n, device, [], []
-        codes = DTYPE_CODES
-        ptr, numel, dtype = [], [], []
-        for g in grads:
-            if g.layout is not torch.strided or g.dtype not in codes:
-                raise ValueError("gradients are dense float32, bfloat16 or float16 tensors, got %s, %s" % (g.layout, g.dtype))
-            if g.device != device:
-                raise ValueError("all gradients lie on one device, got %s and %s" % (device, g.device))
-            if not g.is_contiguous() and _flat(g) is None:
-                if writable and any(st == 0 and sz > 1 for sz, st in zip(g.shape, g.stride())):
-                    raise ValueError("a gradient that was expanded cannot be scaled in place")
-                c = g.contiguous()
-                self.back.append((g, c))
-                g = c
-            keep.append(g)
-            ptr.append(g.data_ptr())
-            numel.append(g.numel())
-            dtype.append(codes[g.dtype])
-        self.keep = keep
-        self.ptr, self.numel, self.dtype = (ctypes.c_uint64 * n)(*ptr), (ctypes.c_int64 * n)(*numel), (ctypes.c_int32 * n)(*dtype)
+    def __init__(self, tensors):
+        self.n, self.back = len(tensors), []
+        self.x, self.numel, self.dtype = (ctypes.c_uint64 * self.n)(), (ctypes.c_int64 * self.n)(), (ctypes.c_int32 * self.n)()
+        for i in load_tensorlist().describe(tensors, ctypes.addressof(self.x), ctypes.addressof(self.numel), ctypes.addressof(self.dtype)):
+            self.back.append((tensors[i], tensors[i].contiguous()))
+            self.x[i] = self.back[-1][1].data_ptr()
+        self.device = tensors[0].device
 
     def sumsq(self, stream):
-        """(partial sums, how many): the workspace is this call's own"""
-        lib = load_library()
-        room = lib.pinn_grad_norm_partials(self.n)
-        partials = torch.empty(max(1, room), dtype=torch.float64, device=self.device)
-        count = ctypes.c_int32()
-        _check(lib.pinn_grad_sumsq(self.ptr, self.numel, self.dtype, self.n, partials.data_ptr(), room, ctypes.byref(count), stream), "pinn_grad_sumsq")
-        return partials, count.value
+        return _sumsq(self.x, self.numel, self.dtype, self.n, self.device, stream)
 
 
-def _tensor_list(tensors):
+def _sumsq(x, numel, dtype, n, device, stream):
+    """(partial sums, how many): the workspace is the call's own"""
+    lib = load_library()
+    room = lib.pinn_grad_norm_partials(n)
+    partials = torch.empty(room, dtype=torch.float64, device=device)
+    count = ctypes.c_int32()
+    _check(lib.pinn_grad_sumsq(x, numel, dtype, n, partials.data_ptr(), room, ctypes.byref(count), stream), "pinn_grad_sumsq")
+    return partials, count.value
+
+
+def _tensors(tensors):
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    for t in tensors:
-        if not torch.is_tensor(t):
-            raise TypeError("expected tensors, got %s" % type(t).__name__)
-    if tensors and not tensors[0].is_cuda:
+    if tensors and torch.is_tensor(tensors[0]) and not tensors[0].is_cuda:
         raise NativeError("the tensors are on %s: pde_amd needs an AMD GPU; there is no CPU fallback" % tensors[0].device)
     return tensors
 
@@ -193,13 +180,12 @@ def grad_norm(tensors):
     """2-norm over all elements of all `tensors` (one, or an iterable; float32, bfloat16, float16, mixed as they come): a 0-dim
     float32 tensor on their device.  Squares and sums are float64, in a fixed order: the same inputs give the same bits, and
     no float32 value overflows or vanishes on the way.  An empty list gives 0."""
-    tensors = _tensor_list(tensors)
+    tensors = _tensors(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    dev = tensors[0].device
-    lst = _GradList(tensors, dev, writable=False)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    with _on(dev):
+    lst = _TensorList(tensors)
+    norm = torch.empty((), dtype=torch.float32, device=lst.device)
+    with _on(lst.device):
         stream = _cur_stream(norm)
         partials, n = lst.sumsq(stream)
         _check(load_library().pinn_grad_norm(partials.data_ptr(), n, norm.data_ptr(), stream), "pinn_grad_norm")
@@ -215,28 +201,29 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm is %r: 0 or more is needed" % max_norm)
-    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
-    grads = _tensor_list([p.grad for p in parameters if p.grad is not None])
+    native = load_tensorlist()
+    grads = _tensors(native.grads([parameters] if torch.is_tensor(parameters) else list(parameters)))
     if not grads:
         return torch.tensor(0.0)
-    dev = grads[0].device
-    lst = _GradList(grads, dev, writable=True)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
+    lst = _TensorList(grads)
+    if any(0 in (st for sz, st in zip(g.shape, g.stride()) if sz > 1) for g, _ in lst.back):
+        raise ValueError("a gradient that was expanded cannot be scaled in place")
+    norm = torch.empty((), dtype=torch.float32, device=lst.device)
     lib = load_library()
-    with _on(dev):
+    with _on(lst.device):
         stream = _cur_stream(norm)
         partials, n = lst.sumsq(stream)
         if error_if_nonfinite:
             _check(lib.pinn_grad_norm(partials.data_ptr(), n, norm.data_ptr(), stream), "pinn_grad_norm")
             if not torch.isfinite(norm):
                 raise RuntimeError("the gradients' norm is %s: they were not clipped" % norm.item())
-        rc = lib.pinn_grad_clip(lst.ptr, lst.numel, lst.dtype, lst.n, partials.data_ptr(), n, max_norm, norm.data_ptr(), stream)
+        rc = lib.pinn_grad_clip(lst.x, lst.numel, lst.dtype, lst.n, partials.data_ptr(), n, max_norm, norm.data_ptr(), stream)
         if rc == ERR_OVERLAP:
             raise ValueError("two of the gradients share memory: scaling them in place would scale it twice")
         _check(rc, "pinn_grad_clip")
         for g, c in lst.back:
             g.copy_(c)
-    torch.autograd.graph.increment_version(grads)
+    native.written(grads, 0)
     return norm
 
 
@@ -278,7 +265,7 @@ class GroupedAdamW(torch.optim.Optimizer):
         if self.device.type != "cuda":
             raise NativeError("GroupedAdamW needs parameters on an AMD GPU, got %s; there is no CPU fallback (use torch.optim.AdamW)" % self.device)
         self._check_params()
-        self.lib = load_library()
+        self.lib, self._native = load_library(), load_tensorlist()
         self._plan(bool(master_weights))
         self._planned = True
 
@@ -330,17 +317,28 @@ class GroupedAdamW(torch.optim.Optimizer):
         self.device_state[:, 0] = 0.0
         self._ticket = torch.zeros(ADAMW_TICKET_WORDS, dtype=torch.int32, device=dev)
         self._norm = torch.zeros((), dtype=torch.float32, device=dev)
-        self._launches, first = [], 0
+        # launches: consecutive runs of the parameters sorted by group and type
+        plan, first = [], 0
         for grp in self.param_groups:
             rows = range(first, first + len(grp["params"]))
             first += len(grp["params"])
             for dt in DTYPE_CODES:
-                mine = [i for i in rows if self._params[i].dtype == dt and self._params[i].numel()]
-                for a in range(0, len(mine), ADAMW_MAX_TENSORS):
-                    self._launches.append(self._launch(grp, dt, mine[a:a + ADAMW_MAX_TENSORS]))
+                mine = [i for i in rows if self._params[i].dtype == dt]
+                plan += [(grp, dt, mine[a:a + ADAMW_MAX_TENSORS]) for a in range(0, len(mine), ADAMW_MAX_TENSORS)]
+        order = [i for _, _, rows in plan for i in rows]
+        n = len(order)
+        self._ordered = [self._params[i] for i in order]
+        self._numel = (ctypes.c_int64 * n)(*(p.numel() for p in self._ordered))
+        self._dtype = (ctypes.c_int32 * n)(*(DTYPE_CODES[p.dtype] for p in self._ordered))
+        self._p, self._g, self._count = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)(), (ctypes.c_int64 * n)()
+        self._gather_args = tuple(ctypes.addressof(x) for x in (self._numel, self._dtype, self._p, self._g, self._count))
+        self._launches, first = [], 0
+        for grp, dt, rows in plan:
+            self._launches.append(self._launch(grp, dt, rows, first))
+            first += len(rows)
 
-    def _launch(self, grp, dtype, rows):
-        parts, chunk = [], ADAMW_CHUNK32 if self.state_bits == 32 else ADAMW_CHUNK8
+    def _launch(self, grp, dtype, rows, first):
+        parts, chunk = [np.zeros(0, dtype=ADAMW_CHUNK_DTYPE)], ADAMW_CHUNK32 if self.state_bits == 32 else ADAMW_CHUNK8
         for k, i in enumerate(rows):
             base = np.arange(0, self._params[i].numel(), chunk, dtype=np.int64)
             part = np.zeros(len(base), dtype=ADAMW_CHUNK_DTYPE)
@@ -352,14 +350,15 @@ class GroupedAdamW(torch.optim.Optimizer):
         where = torch.tensor(rows, dtype=torch.int32, device=self.device)
         d = PinnAdamWGroup()
         d.chunks, d.rows, d.n_chunks, d.n_tensors = chunks.data_ptr(), where.data_ptr(), len(parts), len(rows)
-        d.dtype, d.state_bits, d.skip_nonfinite = DTYPE_CODES[dtype], self.state_bits, int(self.skip_nonfinite)
+        d.dtype, d.state_bits = DTYPE_CODES[dtype], self.state_bits
         d.exp_avg, d.exp_avg_sq, d.device_state, d.ticket = (t.data_ptr() for t in (self.exp_avg, self.exp_avg_sq, self.device_state, self._ticket))
         if self.state_bits == 8:
             d.exp_avg_scale, d.exp_avg_sq_scale = self.exp_avg_scale.data_ptr(), self.exp_avg_sq_scale.data_ptr()
         if self.master is not None and dtype != torch.float32:
             d.master = self.master.data_ptr()
-        d.max_norm = -1.0 if self.max_norm is None else self.max_norm
-        return dict(grp=grp, desc=d, rows=rows, p=(ctypes.c_uint64 * len(rows))(), g=(ctypes.c_uint64 * len(rows))(), tables=(chunks, where))
+        d.norm = self._norm.data_ptr()
+        return dict(grp=grp, desc=d, ref=ctypes.byref(d), rows=rows, p=ctypes.addressof(self._p) + 8 * first,
+                    g=ctypes.addressof(self._g) + 8 * first, tables=(chunks, where))
 
     @torch.no_grad()
     def sync_master(self):
@@ -419,44 +418,30 @@ class GroupedAdamW(torch.optim.Optimizer):
             for name in self._held():
                 getattr(self, name).copy_(fused[name])
 
-    def _gradient(self, p):
-        """`p.grad` in `p`'s order in memory"""
-        g = p.grad
-        if g.layout is not torch.strided:
-            raise ValueError("GroupedAdamW takes dense gradients, got %s" % g.layout)
-        if g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
-            raise ValueError("the gradient is %s %s on %s, its parameter %s %s on %s" % (tuple(g.shape), g.dtype, g.device, tuple(p.shape), p.dtype, p.device))
-        if g.stride() != p.stride():
-            g = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
-        return g
-
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        params, grads = self._params, []
-        for i, p in enumerate(params):
-            if p.grad is None:
-                grads.append(None)
-                continue
-            grads.append(self._gradient(p))
         hyper = {id(grp): self._hyper(grp) for grp in self.param_groups}
-        given = [g for g in grads if g is not None and g.numel()]
+        given, other = self._native.gather(self._ordered, *self._gather_args)
         if not given:
             return loss
+        keep = []
+        for i in other:                                 # a gradient in another order in memory than its parameter
+            p = self._ordered[i]
+            keep.append(torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(p.grad.detach()))
+            self._g[i] = keep[-1].data_ptr()
         with _on(self.device):
             stream = _cur_stream(self._norm)
             partials, n_partials = None, 0
             if self.max_norm is not None or self.skip_nonfinite:
-                partials, n_partials = _GradList(given, self.device, writable=False).sumsq(stream)
+                partials, n_partials = _sumsq(self._g, self._count, self._dtype, len(self._ordered), self.device, stream)
             for launch in self._launches:
-                d, rows = launch["desc"], launch["rows"]
-                launch["p"][:] = [params[i].data_ptr() for i in rows]
-                launch["g"][:] = [0 if grads[i] is None else grads[i].data_ptr() for i in rows]
+                d = launch["desc"]
                 d.lr, d.beta1, d.beta2, d.eps, d.weight_decay = hyper[id(launch["grp"])]
-                d.partials, d.n_partials, d.norm = partials.data_ptr() if n_partials else None, n_partials, self._norm.data_ptr()
-                _check(self.lib.pinn_adamw_group_step(ctypes.byref(d), launch["p"], launch["g"], stream), "pinn_adamw_group_step")
-        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+                d.partials, d.n_partials = partials.data_ptr() if n_partials else None, n_partials
+                d.max_norm, d.skip_nonfinite = -1.0 if self.max_norm is None else self.max_norm, self.skip_nonfinite
+                _check(self.lib.pinn_adamw_group_step(launch["ref"], launch["p"], launch["g"], stream), "pinn_adamw_group_step")
+        self._native.written(self._ordered, self._gather_args[4])
         return loss

@@ -147,3 +147,58 @@ def test_options_that_need_the_grouped_step():
     m.adam_impl = "grouped"
     with pytest.raises(NativeError, match="no CPU fallback"):
         m.train(1, LBFGS_max_iter=0)
+
+
+def test_lists_of_tensors():
+    """csrc/tensorlist.cpp on CPU tensors: what it reads, which gradients it hands back, what it refuses"""
+    import ctypes as C
+    from pde_amd._native import load_tensorlist
+    native = load_tensorlist()
+    ps = [torch.nn.Parameter(x) for x in (torch.randn(3, 5), torch.randn(0), torch.randn(7, 4).t(), torch.randn(6).half(), torch.randn(1, 9), torch.randn(2).bfloat16())]
+    n = len(ps)
+    numel, dtype = (C.c_int64 * n)(*(p.numel() for p in ps)), (C.c_int32 * n)(0, 0, 0, 2, 0, 1)
+    p, g, count = (C.c_uint64 * n)(), (C.c_uint64 * n)(), (C.c_int64 * n)()
+
+    def gather():
+        return native.gather(ps, *(C.addressof(x) for x in (numel, dtype, p, g, count)))
+    assert gather() == (0, []) and list(g) == [0] * n and list(count) == [0] * n
+    for q in ps[:5]:
+        q.grad = torch.ones_like(q)
+    assert gather() == (4, []) and list(count) == [15, 0, 28, 6, 9, 0]
+    assert list(p) == [q.data_ptr() for q in ps] and g[0] == ps[0].grad.data_ptr() and g[1] == g[5] == 0
+    ps[2].grad = torch.ones(4, 7)                                              # another order than its parameter's
+    ps[4].grad = torch.ones(9, 1).t()                                          # another stride of a dimension of one element: the same order
+    assert gather() == (4, [2]) and g[2] == 0 and g[4] == ps[4].grad.data_ptr()
+    before = [q._version for q in ps]
+    native.written(ps, C.addressof(count))
+    assert [q._version - b for q, b in zip(ps, before)] == [1, 0, 1, 1, 1, 0]
+    assert [x.data_ptr() for x in native.grads(ps)] == [q.grad.data_ptr() for q in ps[:5]]
+    dtype[3] = 1
+    with pytest.raises(ValueError, match="parameter 3 is not what it was"):
+        gather()
+    dtype[3] = 2
+    ps[0].data = torch.randn(3, 6)
+    with pytest.raises(ValueError, match="parameter 0"):
+        gather()
+    ps[0].data = torch.randn(3, 5)
+    ps[0].grad.data = torch.ones(5, 3)
+    with pytest.raises(ValueError, match="gradient of parameter 0"):
+        gather()
+    ps[0].grad = None
+    ps[0].grad = torch.sparse_coo_tensor(torch.tensor([[0], [1]]), torch.tensor([1.0]), (3, 5))
+    with pytest.raises(ValueError, match="gradient of parameter 0"):
+        gather()
+    x = (C.c_uint64 * 3)()
+
+    def describe(ts):
+        return native.describe(ts, C.addressof(x), C.addressof(numel), C.addressof(dtype))
+    a = torch.randn(4, 6)
+    assert describe([a, a.t(), a[:, ::2]]) == [2] and list(x)[:2] == [a.data_ptr()] * 2 and list(numel)[:3] == [24, 24, 12]
+    for bad in (a.double(), a.long(), a.to_sparse()):
+        with pytest.raises(ValueError, match="tensor 1"):
+            describe([a, bad])
+    with pytest.raises(ValueError, match="one device"):
+        describe([a, torch.empty(2, device="meta")])
+    for call in (lambda: describe([a, 3]), lambda: native.grads([a, None]), lambda: native.gather([None] * 6, 0, 0, 0, 0, 0), lambda: native.grads((a,)), lambda: describe((a,))):
+        with pytest.raises(TypeError):
+            call()
