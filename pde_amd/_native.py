@@ -169,7 +169,8 @@ def _split_xt(x, t):
 
 
 def _cur_stream(t):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    """torch's current stream on `t`'s device (read raw: building the Stream object takes 1.8 us)"""
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(t.device.index))
 
 
 def data_loss(out, tgt0, n0, nb, dirichlet, losses=None):

@@ -15,6 +15,7 @@ import ctypes
 
 import numpy as np
 import torch
+import torch.optim.optimizer as _hooks
 
 from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, DTYPE_CODES, ERR_OVERLAP, NativeError, PinnAdamWGroup, _check, _cur_stream, _on, load_library,
                       load_tensorlist)
@@ -150,7 +151,8 @@ class _TensorList:
         self.n, self.back = len(tensors), []
         self.x, self.numel, self.dtype = (ctypes.c_uint64 * self.n)(), (ctypes.c_int64 * self.n)(), (ctypes.c_int32 * self.n)()
         for i in load_tensorlist().describe(tensors, ctypes.addressof(self.x), ctypes.addressof(self.numel), ctypes.addressof(self.dtype)):
-            self.back.append((tensors[i], tensors[i].contiguous()))
+            t = tensors[i].detach()
+            self.back.append((t, t.contiguous()))
             self.x[i] = self.back[-1][1].data_ptr()
         self.device = tensors[0].device
 
@@ -175,7 +177,6 @@ def _tensors(tensors):
     return tensors
 
 
-@torch.no_grad()
 def grad_norm(tensors):
     """2-norm over all elements of all `tensors` (one, or an iterable; float32, bfloat16, float16, mixed as they come): a 0-dim
     float32 tensor on their device.  Squares and sums are float64, in a fixed order: the same inputs give the same bits, and
@@ -192,7 +193,6 @@ def grad_norm(tensors):
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     """Scales the gradients of `parameters` in place so that their global 2-norm is at most `max_norm`, and returns the norm
     they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 160 tensors, without a copy of the
@@ -373,12 +373,12 @@ class GroupedAdamW(torch.optim.Optimizer):
         """norm of the gradients of the last step (0-dim float32, overwritten by the next); steps without `max_norm` or `skip_nonfinite` do not form it"""
         return self._norm
 
-    @torch.no_grad()
     def moments(self):
         """(exp_avg, exp_avg_sq) as flat float32 tensors in the order of the flat state: the buffers themselves, or with 8 bits what they stand for."""
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
-        m, v = (torch.empty(self.state_numel, dtype=torch.float32, device=self.device) for _ in range(2))
+        m = torch.empty(self.state_numel, dtype=torch.float32, device=self.device)
+        v = torch.empty_like(m)
         with _on(self.device):
             _check(self.lib.pinn_adamw_moments(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.exp_avg_scale.data_ptr(),
                                                self.exp_avg_sq_scale.data_ptr(), m.data_ptr(), v.data_ptr(), self.state_numel, _cur_stream(m)),
@@ -419,6 +419,17 @@ class GroupedAdamW(torch.optim.Optimizer):
                 getattr(self, name).copy_(fused[name])
 
     def step(self, closure=None):
+        """One step of every parameter that has a gradient; `closure` is called first, as in torch, and its loss returned."""
+        # torch wraps every optimizer's `step` for its profiler's label and for step hooks, which takes as long as all the rest of a small
+        # net's step (6.7 us): here the wrapper is used where one of them is
+        if (self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _hooks._global_optimizer_pre_hooks
+                or _hooks._global_optimizer_post_hooks or torch.autograd._profiler_enabled()):
+            return self._hooked_step(closure)
+        return self._step(closure)
+
+    step.hooked = True
+
+    def _step(self, closure):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -445,3 +456,5 @@ class GroupedAdamW(torch.optim.Optimizer):
                 _check(self.lib.pinn_adamw_group_step(launch["ref"], launch["p"], launch["g"], stream), "pinn_adamw_group_step")
         self._native.written(self._ordered, self._gather_args[4])
         return loss
+
+    _hooked_step = torch.optim.Optimizer.profile_hook_step(_step)

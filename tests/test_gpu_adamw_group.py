@@ -343,6 +343,29 @@ def test_step_on_another_stream_and_closure():
     assert opt.device_state[:, 0].tolist() == [2.0 if i == 9 else 0.0 for i in range(len(params))]
 
 
+def test_hooks_profiler_and_scheduler():
+    """what torch's wrapper of `step` serves: step hooks, the profiler's label, learning-rate schedulers"""
+    params = params_of(make(SIZES, torch.float32, 62))
+    opt = GroupedAdamW(params, **HYPER)
+    for p, g in zip(params, make(SIZES, torch.float32, 63)):
+        p.grad = g
+    seen = []
+    hooks = [opt.register_step_pre_hook(lambda o, a, k: seen.append("pre")), opt.register_step_post_hook(lambda o, a, k: seen.append("post"))]
+    opt.step()
+    assert seen == ["pre", "post"]
+    for h in hooks:
+        h.remove()
+    opt.step()
+    assert seen == ["pre", "post"] and opt.device_state[0, 0] == 2
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        opt.step()
+    assert any("Optimizer.step#GroupedAdamW.step" in e.key for e in prof.key_averages())
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    opt.step()
+    sched.step()
+    assert opt.param_groups[0]["lr"] == HYPER["lr"] / 2 and opt.device_state[0, 0] == 4
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_state_dict_continues(bits):
     def model():
