@@ -275,6 +275,7 @@ int pinn_adam_step(float *theta, const float *grad, float *exp_avg, float *exp_a
 #define PINN_ADAMW_CHUNK8 2048       /* the same with 8-bit moments */
 #define PINN_ADAMW_MAX_TENSORS 240   /* tensors per call: their addresses are launch arguments */
 #define PINN_ADAMW_TICKET_WORDS 2080 /* words of the ticket buffer */
+#define PINN_NORM_TENSORS 256       /* tensors per launch of the norm */
 #define PINN_NORM_PARTIALS 1024      /* most partial sums per launch of pinn_grad_sumsq */
 
 typedef struct {                     /* PINN_ADAMW_CHUNK32 or _CHUNK8 elements of one tensor, or the rest of it */
@@ -318,11 +319,12 @@ int pinn_adamw_moments(const uint8_t *exp_avg, const uint8_t *exp_avg_sq, const 
 int64_t pinn_grad_norm_partials(int32_t n_tensors);
 int pinn_grad_sumsq(const void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, double *partials,
                     int64_t n_reserved, int32_t *n_partials, void *stream);
-/* *norm = sqrt of their sum */
-int pinn_grad_norm(const double *partials, int32_t n_partials, float *norm, void *stream);
-/* the same, and grads *= min(1, max_norm / (norm + 1e-6)) in place; no two tensors may overlap */
-int pinn_grad_clip(void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, const double *partials,
-                   int32_t n_partials, double max_norm, float *norm, void *stream);
+/* *norm = the 2-norm over the list; `partials`, `n_reserved`: room as for pinn_grad_sumsq */
+int pinn_grad_norm(const void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, double *partials,
+                   int64_t n_reserved, float *norm, void *stream);
+/* the same, and grads *= min(1, max_norm / (norm + 1e-6)) in place; PINN_ERR_OVERLAP if two tensors share memory */
+int pinn_grad_clip(void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, double *partials,
+                   int64_t n_reserved, double max_norm, float *norm, void *stream);
 
 const char *pinn_error_string(int code);
 

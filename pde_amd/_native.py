@@ -110,8 +110,8 @@ def load_library():
     lib.pinn_grad_norm_partials.argtypes = [i32]
     lib.pinn_grad_norm_partials.restype = i64
     lib.pinn_grad_sumsq.argtypes = [vp, vp, vp, i32, vp, i64, ctypes.POINTER(i32), vp]
-    lib.pinn_grad_norm.argtypes = [vp, i32, vp, vp]
-    lib.pinn_grad_clip.argtypes = [vp, vp, vp, i32, vp, i32, ctypes.c_double, vp, vp]
+    lib.pinn_grad_norm.argtypes = [vp, vp, vp, i32, vp, i64, vp, vp]
+    lib.pinn_grad_clip.argtypes = [vp, vp, vp, i32, vp, i64, ctypes.c_double, vp, vp]
     lib.pinn_error_string.argtypes = [ctypes.c_int]
     lib.pinn_error_string.restype = ctypes.c_char_p
     _lib = lib

@@ -22,6 +22,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/pinnjet.h"
 
@@ -35,7 +36,7 @@ constexpr int kMaxTensors = PINN_ADAMW_MAX_TENSORS;
 // at once cost memory bandwidth.  float32 moments, 240M float32 weights (28 bytes each): 8 workgroups of 2048 elements 1186 us, 5 of them 1138,
 // 5 of 1024 elements 1099, 6 of 1024 elements 1082 (6.2 TB/s), 3 of 1024 elements 1394.  8-bit moments, 240M float32 weights (16 bytes): free 673 us, 5 workgroups 653.
 constexpr unsigned kPace32 = 27000, kPace8 = 32000;
-constexpr int kNormTensors = 160;
+constexpr int kNormTensors = PINN_NORM_TENSORS;
 constexpr int kNormChunk = 8192;
 constexpr int kMaxPartials = PINN_NORM_PARTIALS;
 static_assert(sizeof(PinnAdamWChunk) == 32 && sizeof(PinnAdamWGroup) == 168, "the callers' layouts");
@@ -489,11 +490,12 @@ __global__ __launch_bounds__(kThreads) void k_moments(const uint8_t *m, const ui
 // Workgroup b always takes the same chunks and its sum has its own place, so the norm is the same bits on every run.
 struct NormArgs {
     void *x[kNormTensors];
-    int64_t numel[kNormTensors];
     int32_t first_chunk[kNormTensors + 1];
+    uint16_t tail[kNormTensors];                // elements of a tensor's last chunk, 1 .. kNormChunk
     uint8_t dtype[kNormTensors];
     int32_t n_tensors, first_partial;
 };
+static_assert(sizeof(NormArgs) + 48 <= 4096, "a launch's arguments");
 
 __device__ inline int find_tensor(const NormArgs &a, int64_t ch)
 {
@@ -538,8 +540,8 @@ __global__ __launch_bounds__(kThreads) void k_grad_sumsq(const NormArgs a, doubl
     const int64_t n_chunks = a.first_chunk[a.n_tensors];
     for (int64_t ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
         const int k = find_tensor(a, ch);
-        const int64_t base = (ch - a.first_chunk[k]) * kNormChunk, left = a.numel[k] - base;
-        const int count = left < kNormChunk ? (int)left : kNormChunk;
+        const int64_t base = (ch - a.first_chunk[k]) * kNormChunk;
+        const int count = ch + 1 == a.first_chunk[k + 1] ? a.tail[k] : kNormChunk;
         if (a.dtype[k] == PINN_F32) s += chunk_sumsq((const float *)a.x[k] + base, count);
         else if (a.dtype[k] == PINN_BF16) s += chunk_sumsq((const __bf16 *)a.x[k] + base, count);
         else s += chunk_sumsq((const _Float16 *)a.x[k] + base, count);
@@ -591,12 +593,53 @@ __global__ __launch_bounds__(kThreads) void k_grad_clip(const NormArgs a, const 
     const int64_t n_chunks = a.first_chunk[a.n_tensors];
     for (int64_t ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
         const int k = find_tensor(a, ch);
-        const int64_t base = (ch - a.first_chunk[k]) * kNormChunk, left = a.numel[k] - base;
-        const int count = left < kNormChunk ? (int)left : kNormChunk;
+        const int64_t base = (ch - a.first_chunk[k]) * kNormChunk;
+        const int count = ch + 1 == a.first_chunk[k + 1] ? a.tail[k] : kNormChunk;
         if (a.dtype[k] == PINN_F32) chunk_scale((float *)a.x[k] + base, count, f);
         else if (a.dtype[k] == PINN_BF16) chunk_scale((__bf16 *)a.x[k] + base, count, f);
         else chunk_scale((_Float16 *)a.x[k] + base, count, f);
     }
+}
+
+// Few elements: ONE workgroup forms the norm and, with max_norm >= 0, scales, a wave to a tensor at a time.  A launch is 3.7 us at the
+// host, so for a small net the second one is a third of the call.
+constexpr int kSmallThreads = 1024, kSmallTensors = 64;
+constexpr int64_t kSmallElements = 16384;
+
+template <class T, class F>
+__device__ inline void wave_over(T *x, int n, F f)
+{
+#pragma unroll 4
+    for (int i = threadIdx.x & 63; i < n; i += 64) f(x[i]);
+}
+
+template <class F>
+__device__ inline void waves_over(const NormArgs &a, F f)
+{
+    for (int k = threadIdx.x >> 6; k < a.n_tensors; k += kSmallThreads / 64) {
+        const int n = (a.first_chunk[k + 1] - a.first_chunk[k] - 1) * kNormChunk + a.tail[k];
+        if (a.dtype[k] == PINN_F32) wave_over((float *)a.x[k], n, f);
+        else if (a.dtype[k] == PINN_BF16) wave_over((__bf16 *)a.x[k], n, f);
+        else wave_over((_Float16 *)a.x[k], n, f);
+    }
+}
+
+__global__ __launch_bounds__(kSmallThreads) void k_norm_small(const NormArgs a, double max_norm, float *norm_out)
+{
+    __shared__ double part[kSmallThreads / 64];
+    double s = 0.0;
+    waves_over(a, [&](auto &x) { s = fma((double)(float)x, (double)(float)x, s); });
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0;
+    for (int w = 0; w < kSmallThreads / 64; ++w) s += part[w];
+    const double norm = sqrt(s);
+    if (threadIdx.x == 0) *norm_out = (float)norm;
+    if (max_norm < 0.0) return;
+    const float f = (float)clip_factor(norm, max_norm);
+    if (f == 1.0f) return;
+    waves_over(a, [&](auto &x) { x = (std::remove_reference_t<decltype(x)>)((float)x * f); });
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
@@ -634,7 +677,7 @@ struct NormPlan {
             if (chunks + more > INT32_MAX) break;
             const int k = a.n_tensors++;
             a.x[k] = x[next];
-            a.numel[k] = numel[next];
+            a.tail[k] = (uint16_t)(numel[next] - (more - 1) * kNormChunk);
             a.dtype[k] = (uint8_t)dtype[next];
             a.first_chunk[k] = (int32_t)chunks;
             chunks += more;
@@ -667,12 +710,39 @@ int check_apart(void *const *x, const int64_t *numel, const int32_t *dtype, int3
     int m = 0;
     for (int32_t i = 0; i < n; ++i)
         if (numel[i] > 0) s[m++] = {(uintptr_t)x[i], (uintptr_t)x[i] + (uintptr_t)numel[i] * (dtype[i] == PINN_F32 ? 4 : 2)};
-    std::sort(s, s + m, [](const Span &a, const Span &b) { return a.begin < b.begin; });
+    const auto before = [](const Span &a, const Span &b) { return a.begin < b.begin; };
+    if (!std::is_sorted(s, s + m, before)) std::sort(s, s + m, before);
     int rc = PINN_OK;
     for (int i = 1; i < m; ++i)
         if (s[i].begin < s[i - 1].end) rc = PINN_ERR_OVERLAP;
     free(s);
     return rc;
+}
+
+// the whole list in one workgroup's launch, if it is small enough
+bool small_list(NormArgs &a, void *const *x, const int64_t *numel, const int32_t *dtype, int n)
+{
+    int64_t total = 0;
+    for (int i = 0; i < n; ++i) {
+        total += numel[i] < kSmallElements ? numel[i] : kSmallElements + 1;
+        if (total > kSmallElements) return false;
+    }
+    NormPlan plan;
+    plan.advance(a, x, numel, dtype, n);
+    return plan.next == n && a.n_tensors <= kSmallTensors;
+}
+
+int launch_sumsq(const void *const *grads, const int64_t *numel, const int32_t *dtype, int n_tensors, double *partials, int64_t n_reserved,
+                 int32_t *n_partials, void *stream)
+{
+    NormArgs a;
+    NormPlan plan;
+    while (plan.advance(a, (void *const *)grads, numel, dtype, n_tensors)) {
+        if (plan.partials > n_reserved) return PINN_ERR_TOO_LARGE;
+        hipLaunchKernelGGL(k_grad_sumsq, dim3(plan.grid), dim3(kThreads), 0, (hipStream_t)stream, a, partials);
+        *n_partials = plan.partials;
+    }
+    return launch_error();
 }
 
 }  // namespace
@@ -687,46 +757,50 @@ extern "C" int pinn_grad_sumsq(const void *const *grads, const int64_t *numel, c
 {
     if (const int rc = check_list(grads, numel, dtype, n_tensors)) return rc;
     if (!n_partials || !partials) return PINN_ERR_NULL;
-    NormArgs a;
-    NormPlan plan;
     *n_partials = 0;
-    while (plan.advance(a, (void *const *)grads, numel, dtype, n_tensors)) {
-        if (plan.partials > n_reserved) return PINN_ERR_TOO_LARGE;
-        hipLaunchKernelGGL(k_grad_sumsq, dim3(plan.grid), dim3(kThreads), 0, (hipStream_t)stream, a, partials);
-        *n_partials = plan.partials;
-    }
-    // Whoever takes the partial sums adds them up in each of its workgroups: up to kThreads of them that is one load a thread, beyond it a
-    // launch of its own (3 us) is less than what thousands of workgroups spend on it.
-    if (*n_partials > kThreads) {
+    if (const int rc = launch_sumsq(grads, numel, dtype, n_tensors, partials, n_reserved, n_partials, stream)) return rc;
+    // Every workgroup of the step adds the partial sums up for itself.  Up to two loads a thread that costs less than a launch (5M
+    // weights); beyond, there are thousands of workgroups and they are added once (60M float32 weights, 8-bit moments: 285 -> 255 us).
+    if (*n_partials > 2 * kThreads) {
         hipLaunchKernelGGL(k_fold, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, partials, *n_partials);
         *n_partials = 1;
     }
     return launch_error();
 }
 
-extern "C" int pinn_grad_norm(const double *partials, int32_t n_partials, float *norm, void *stream)
+extern "C" int pinn_grad_norm(const void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, double *partials,
+                              int64_t n_reserved, float *norm, void *stream)
 {
-    if (!partials || !norm) return PINN_ERR_NULL;
-    if (n_partials < 0) return PINN_ERR_INVALID_DESC;
+    if (const int rc = check_list(grads, numel, dtype, n_tensors)) return rc;
+    if (!norm || !partials) return PINN_ERR_NULL;
+    NormArgs a;
+    if (small_list(a, (void *const *)grads, numel, dtype, n_tensors)) {
+        hipLaunchKernelGGL(k_norm_small, dim3(1), dim3(kSmallThreads), 0, (hipStream_t)stream, a, -1.0, norm);
+        return launch_error();
+    }
+    int32_t n_partials = 0;
+    if (const int rc = launch_sumsq(grads, numel, dtype, n_tensors, partials, n_reserved, &n_partials, stream)) return rc;
     hipLaunchKernelGGL(k_norm_of, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, partials, (int)n_partials, norm);
     return launch_error();
 }
 
-extern "C" int pinn_grad_clip(void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, const double *partials,
-                              int32_t n_partials, double max_norm, float *norm, void *stream)
+extern "C" int pinn_grad_clip(void *const *grads, const int64_t *numel, const int32_t *dtype, int32_t n_tensors, double *partials,
+                              int64_t n_reserved, double max_norm, float *norm, void *stream)
 {
     if (const int rc = check_list((const void *const *)grads, numel, dtype, n_tensors)) return rc;
-    if (!partials || !norm) return PINN_ERR_NULL;
-    if (n_partials < 0 || !(max_norm >= 0.0)) return PINN_ERR_INVALID_DESC;
+    if (!norm || !partials) return PINN_ERR_NULL;
+    if (!(max_norm >= 0.0)) return PINN_ERR_INVALID_DESC;
     if (const int rc = check_apart(grads, numel, dtype, n_tensors)) return rc;
     NormArgs a;
-    NormPlan plan;
-    float *out = norm;
-    while (plan.advance(a, grads, numel, dtype, n_tensors)) {
-        hipLaunchKernelGGL(k_grad_clip, dim3(plan.grid), dim3(kThreads), 0, (hipStream_t)stream, a, partials, (int)n_partials, max_norm, out);
-        out = nullptr;
+    if (small_list(a, grads, numel, dtype, n_tensors)) {
+        hipLaunchKernelGGL(k_norm_small, dim3(1), dim3(kSmallThreads), 0, (hipStream_t)stream, a, max_norm, norm);
+        return launch_error();
     }
-    if (out) return pinn_grad_norm(partials, n_partials, norm, stream);   // nothing but empty tensors
+    int32_t n_partials = 0;
+    if (const int rc = launch_sumsq((const void *const *)grads, numel, dtype, n_tensors, partials, n_reserved, &n_partials, stream)) return rc;
+    NormPlan plan;
+    for (float *out = norm; plan.advance(a, grads, numel, dtype, n_tensors); out = nullptr)
+        hipLaunchKernelGGL(k_grad_clip, dim3(plan.grid), dim3(kThreads), 0, (hipStream_t)stream, a, partials, (int)n_partials, max_norm, out);
     return launch_error();
 }
 

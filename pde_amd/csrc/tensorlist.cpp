@@ -110,12 +110,14 @@ PyObject *gather(PyObject *, PyObject *args)
     });
 }
 
-// describe(tensors, x, numel, dtype) -> [indices that are neither contiguous nor another order of the same memory]
+// describe(tensors, of_grads, x, numel, dtype) -> (how many, [(place in the arrays, index) of those that are neither contiguous nor another
+// order of the same memory], index of their GPU); of_grads: the gradients of those tensors that have one
 PyObject *describe(PyObject *, PyObject *args)
 {
     PyObject *list;
+    int of_grads;
     unsigned long long a_x, a_numel, a_dtype;
-    if (!PyArg_ParseTuple(args, "O!KKK", &PyList_Type, &list, &a_x, &a_numel, &a_dtype)) return nullptr;
+    if (!PyArg_ParseTuple(args, "O!pKKK", &PyList_Type, &list, &of_grads, &a_x, &a_numel, &a_dtype)) return nullptr;
     return guarded([&]() -> PyObject * {
         uint64_t *x = (uint64_t *)(uintptr_t)a_x;
         int64_t *numel = (int64_t *)(uintptr_t)a_numel;
@@ -124,66 +126,63 @@ PyObject *describe(PyObject *, PyObject *args)
         PyObject *other = PyList_New(0);
         if (!other) return nullptr;
         c10::Device device(c10::DeviceType::CPU);
+        Py_ssize_t k = 0;
         for (Py_ssize_t i = 0; i < n; ++i) {
             if (!tensor_at(list, i, "tensor")) { Py_DECREF(other); return nullptr; }
-            const at::Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
-            if (i == 0) device = t.device();
+            const at::Tensor &given = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+            const at::Tensor &t = of_grads ? given.grad() : given;
+            if (!t.defined()) continue;
+            if (k == 0) device = t.device();
+            if (!t.is_cuda() && !t.is_meta() && t.device() == device) {
+                static PyObject *native_error = nullptr;
+                if (!native_error) {
+                    PyObject *m = PyImport_ImportModule("pde_amd._native");
+                    native_error = m ? PyObject_GetAttrString(m, "NativeError") : nullptr;
+                    Py_XDECREF(m);
+                }
+                if (native_error)
+                    PyErr_Format(native_error, "tensor %zd is on %s: pde_amd needs an AMD GPU; there is no CPU fallback", i, t.device().str().c_str());
+                Py_DECREF(other);
+                return nullptr;
+            }
             if (!plain(t) || code_of(t) < 0 || t.device() != device) {
                 PyErr_Format(PyExc_ValueError, "tensor %zd: dense float32, bfloat16 or float16 tensors on one device are needed, got %s on %s (the first is on %s)", i,
                              !plain(t) ? "another layout" : c10::toString(t.scalar_type()), t.device().str().c_str(), device.str().c_str());
                 Py_DECREF(other);
                 return nullptr;
             }
-            x[i] = (uint64_t)(uintptr_t)t.data_ptr();
-            numel[i] = t.numel();
-            dtype[i] = code_of(t);
+            x[k] = t.numel() ? (uint64_t)(uintptr_t)t.data_ptr() : 0;
+            numel[k] = t.numel();
+            dtype[k] = code_of(t);
             if (!dense(t)) {
-                PyObject *k = PyLong_FromSsize_t(i);
-                const bool bad = !k || PyList_Append(other, k) != 0;
-                Py_XDECREF(k);
+                PyObject *pair = Py_BuildValue("(nn)", k, i);
+                const bool bad = !pair || PyList_Append(other, pair) != 0;
+                Py_XDECREF(pair);
                 if (bad) { Py_DECREF(other); return nullptr; }
             }
+            ++k;
         }
-        return other;
+        if (k == 0) return Py_BuildValue("(nNO)", k, other, Py_None);
+        return Py_BuildValue("(nNn)", k, other, (Py_ssize_t)device.index());
     });
 }
 
-// grads(params) -> [gradient] of those that have one
-PyObject *grads(PyObject *, PyObject *list)
-{
-    if (!PyList_Check(list)) {
-        PyErr_SetString(PyExc_TypeError, "a list is needed");
-        return nullptr;
-    }
-    return guarded([&]() -> PyObject * {
-        PyObject *out = PyList_New(0);
-        if (!out) return nullptr;
-        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-            if (!tensor_at(list, i, "parameter")) { Py_DECREF(out); return nullptr; }
-            const at::Tensor &g = THPVariable_Unpack(PyList_GET_ITEM(list, i)).grad();
-            if (!g.defined()) continue;
-            PyObject *o = THPVariable_Wrap(g);
-            const bool bad = !o || PyList_Append(out, o) != 0;
-            Py_XDECREF(o);
-            if (bad) { Py_DECREF(out); return nullptr; }
-        }
-        return out;
-    });
-}
-
-// written(tensors, which): the tensors (those with which[i] != 0, an int64 array; 0: all) were written to in place
+// written(tensors, of_grads, which): the tensors (or their gradients) were written to in place; which: int64 array, 0 leaves one out, or
+// no array
 PyObject *written(PyObject *, PyObject *args)
 {
     PyObject *list;
+    int of_grads;
     unsigned long long a_which;
-    if (!PyArg_ParseTuple(args, "O!K", &PyList_Type, &list, &a_which)) return nullptr;
+    if (!PyArg_ParseTuple(args, "O!pK", &PyList_Type, &list, &of_grads, &a_which)) return nullptr;
     return guarded([&]() -> PyObject * {
         const int64_t *which = (const int64_t *)(uintptr_t)a_which;
         for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
             if (which && !which[i]) continue;
             if (!tensor_at(list, i, "tensor")) return nullptr;
-            const at::Tensor &t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            const at::Tensor &given = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+            const at::Tensor &t = of_grads ? given.grad() : given;
+            if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
         }
         Py_RETURN_NONE;
     });
@@ -191,7 +190,6 @@ PyObject *written(PyObject *, PyObject *args)
 
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, nullptr},
                          {"describe", describe, METH_VARARGS, nullptr},
-                         {"grads", grads, METH_O, nullptr},
                          {"written", written, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 

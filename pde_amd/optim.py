@@ -144,86 +144,78 @@ def _flat(t):
 
 
 class _TensorList:
-    """Tensors as the C interface takes them: host arrays of addresses, lengths and types.  `back`: (tensor, copy) of those whose
-    memory has gaps or overlaps, the copy is what the arrays name."""
+    """Tensors, or with `of_grads` the gradients of those that have one, as the C interface takes them: host arrays of addresses, lengths
+    and types.  `back`: (tensor, copy) of those whose memory has gaps or overlaps, the copy is what the arrays name."""
 
-    def __init__(self, tensors):
-        self.n, self.back = len(tensors), []
-        self.x, self.numel, self.dtype = (ctypes.c_uint64 * self.n)(), (ctypes.c_int64 * self.n)(), (ctypes.c_int32 * self.n)()
-        for i in load_tensorlist().describe(tensors, ctypes.addressof(self.x), ctypes.addressof(self.numel), ctypes.addressof(self.dtype)):
-            t = tensors[i].detach()
+    def __init__(self, tensors, of_grads=False):
+        n = len(tensors)
+        self.x, self.numel, self.dtype = (ctypes.c_uint64 * n)(), (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
+        at = ctypes.addressof(self.x), ctypes.addressof(self.numel), ctypes.addressof(self.dtype)
+        self.n, other, index = load_tensorlist().describe(tensors, of_grads, *at)
+        self.device = None if index is None else torch.device("cuda", index)
+        self.back = []
+        for k, i in other:
+            t = tensors[i].grad.detach() if of_grads else tensors[i].detach()
             self.back.append((t, t.contiguous()))
-            self.x[i] = self.back[-1][1].data_ptr()
-        self.device = tensors[0].device
-
-    def sumsq(self, stream):
-        return _sumsq(self.x, self.numel, self.dtype, self.n, self.device, stream)
+            self.x[k] = self.back[-1][1].data_ptr()
 
 
-def _sumsq(x, numel, dtype, n, device, stream):
-    """(partial sums, how many): the workspace is the call's own"""
-    lib = load_library()
-    room = lib.pinn_grad_norm_partials(n)
-    partials = torch.empty(room, dtype=torch.float64, device=device)
-    count = ctypes.c_int32()
-    _check(lib.pinn_grad_sumsq(x, numel, dtype, n, partials.data_ptr(), room, ctypes.byref(count), stream), "pinn_grad_sumsq")
-    return partials, count.value
+def _partials(n, device):
+    """(workspace of the call's own, its length)"""
+    room = load_library().pinn_grad_norm_partials(n)
+    return torch.empty(room, dtype=torch.float64, device=device), room
 
 
-def _tensors(tensors):
-    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    if tensors and torch.is_tensor(tensors[0]) and not tensors[0].is_cuda:
-        raise NativeError("the tensors are on %s: pde_amd needs an AMD GPU; there is no CPU fallback" % tensors[0].device)
-    return tensors
+def _as_list(tensors):
+    return [tensors] if torch.is_tensor(tensors) else list(tensors)
 
 
 def grad_norm(tensors):
     """2-norm over all elements of all `tensors` (one, or an iterable; float32, bfloat16, float16, mixed as they come): a 0-dim
     float32 tensor on their device.  Squares and sums are float64, in a fixed order: the same inputs give the same bits, and
     no float32 value overflows or vanishes on the way.  An empty list gives 0."""
-    tensors = _tensors(tensors)
+    tensors = _as_list(tensors)
     if not tensors:
         return torch.tensor(0.0)
     lst = _TensorList(tensors)
     norm = torch.empty((), dtype=torch.float32, device=lst.device)
+    partials, room = _partials(lst.n, lst.device)
     with _on(lst.device):
-        stream = _cur_stream(norm)
-        partials, n = lst.sumsq(stream)
-        _check(load_library().pinn_grad_norm(partials.data_ptr(), n, norm.data_ptr(), stream), "pinn_grad_norm")
+        _check(load_library().pinn_grad_norm(lst.x, lst.numel, lst.dtype, lst.n, partials.data_ptr(), room, norm.data_ptr(), _cur_stream(norm)),
+               "pinn_grad_norm")
     return norm
 
 
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     """Scales the gradients of `parameters` in place so that their global 2-norm is at most `max_norm`, and returns the norm
-    they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 160 tensors, without a copy of the
-    gradients.  The factor is min(1, max_norm / (norm + 1e-6)); with a norm that is not finite it is 0 or NaN, as there;
-    `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError)."""
+    they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 256 tensors (one for few elements),
+    without a copy of the gradients.  The factor is min(1, max_norm / (norm + 1e-6)); with a norm that is not finite it is 0 or NaN, as
+    there; `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError)."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm is %r: 0 or more is needed" % max_norm)
-    native = load_tensorlist()
-    grads = _tensors(native.grads([parameters] if torch.is_tensor(parameters) else list(parameters)))
-    if not grads:
+    parameters = _as_list(parameters)
+    lst = _TensorList(parameters, of_grads=True)
+    if lst.n == 0:
         return torch.tensor(0.0)
-    lst = _TensorList(grads)
     if any(0 in (st for sz, st in zip(g.shape, g.stride()) if sz > 1) for g, _ in lst.back):
         raise ValueError("a gradient that was expanded cannot be scaled in place")
     norm = torch.empty((), dtype=torch.float32, device=lst.device)
-    lib = load_library()
+    partials, room = _partials(lst.n, lst.device)
+    lib, args = load_library(), (lst.x, lst.numel, lst.dtype, lst.n, partials.data_ptr(), room)
     with _on(lst.device):
         stream = _cur_stream(norm)
-        partials, n = lst.sumsq(stream)
         if error_if_nonfinite:
-            _check(lib.pinn_grad_norm(partials.data_ptr(), n, norm.data_ptr(), stream), "pinn_grad_norm")
+            _check(lib.pinn_grad_norm(*args, norm.data_ptr(), stream), "pinn_grad_norm")
             if not torch.isfinite(norm):
                 raise RuntimeError("the gradients' norm is %s: they were not clipped" % norm.item())
-        rc = lib.pinn_grad_clip(lst.x, lst.numel, lst.dtype, lst.n, partials.data_ptr(), n, max_norm, norm.data_ptr(), stream)
+        rc = lib.pinn_grad_clip(*args, max_norm, norm.data_ptr(), stream)
         if rc == ERR_OVERLAP:
             raise ValueError("two of the gradients share memory: scaling them in place would scale it twice")
         _check(rc, "pinn_grad_clip")
         for g, c in lst.back:
             g.copy_(c)
-    native.written(grads, 0)
+    load_tensorlist().written(parameters, True, 0)
     return norm
 
 
@@ -447,14 +439,18 @@ class GroupedAdamW(torch.optim.Optimizer):
             stream = _cur_stream(self._norm)
             partials, n_partials = None, 0
             if self.max_norm is not None or self.skip_nonfinite:
-                partials, n_partials = _sumsq(self._g, self._count, self._dtype, len(self._ordered), self.device, stream)
+                partials, room = _partials(len(self._ordered), self.device)
+                found = ctypes.c_int32()
+                _check(self.lib.pinn_grad_sumsq(self._g, self._count, self._dtype, len(self._ordered), partials.data_ptr(), room,
+                                                ctypes.byref(found), stream), "pinn_grad_sumsq")
+                n_partials = found.value
             for launch in self._launches:
                 d = launch["desc"]
                 d.lr, d.beta1, d.beta2, d.eps, d.weight_decay = hyper[id(launch["grp"])]
                 d.partials, d.n_partials = partials.data_ptr() if n_partials else None, n_partials
                 d.max_norm, d.skip_nonfinite = -1.0 if self.max_norm is None else self.max_norm, self.skip_nonfinite
                 _check(self.lib.pinn_adamw_group_step(launch["ref"], launch["p"], launch["g"], stream), "pinn_adamw_group_step")
-        self._native.written(self._ordered, self._gather_args[4])
+        self._native.written(self._ordered, False, self._gather_args[4])
         return loss
 
     _hooked_step = torch.optim.Optimizer.profile_hook_step(_step)

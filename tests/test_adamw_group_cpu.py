@@ -111,7 +111,7 @@ def test_c_entries_refuse_without_a_gpu():
     assert lib.pinn_adamw_moments(None, None, None, None, None, None, 0, None) == 0
 
     assert lib.pinn_grad_norm_partials(-1) == INVALID and lib.pinn_grad_norm_partials(0) == 0
-    assert lib.pinn_grad_norm_partials(160) == 1024 and lib.pinn_grad_norm_partials(161) == 2048
+    assert lib.pinn_grad_norm_partials(256) == 1024 and lib.pinn_grad_norm_partials(257) == 2048
     count = ctypes.c_int32()
     n2, f32 = (ctypes.c_int64 * 2)(100, 100), (ctypes.c_int32 * 2)(0, 0)
 
@@ -121,13 +121,18 @@ def test_c_entries_refuse_without_a_gpu():
     assert sums(x=None) == NULL and sums(part=None) == NULL and sums(x=(ctypes.c_uint64 * 2)(16, 0)) == NULL
     assert sums(n=(ctypes.c_int64 * 2)(1, 1 << 62)) == LARGE and sums(room=1) == LARGE
     assert lib.pinn_grad_sumsq(one, n2, f32, 2, 16, 4096, None, None) == NULL
-    assert lib.pinn_grad_norm(None, 1, 16, None) == NULL and lib.pinn_grad_norm(16, -1, 16, None) == INVALID
 
-    def clip(x=one, n=n2, k=2, part=16, m=1.0, out=16, np_=1):
-        return lib.pinn_grad_clip(x, n, f32, k, part, np_, m, out, None)
-    assert clip(m=-1.0) == INVALID and clip(m=float("nan")) == INVALID and clip(np_=-1) == INVALID
+    def norm(x=one, n=n2, dt=f32, k=2, part=16, room=4096, out=16):
+        return lib.pinn_grad_norm(x, n, dt, k, part, room, out, None)
+    big = (ctypes.c_int64 * 2)(1 << 20, 100)
+    assert norm(part=None) == NULL and norm(out=None) == NULL and norm(x=None) == NULL and norm(k=-1) == INVALID and norm(n=big, room=1) == LARGE
+
+    def clip(x=one, n=n2, k=2, part=16, m=1.0, out=16, room=4096):
+        return lib.pinn_grad_clip(x, n, f32, k, part, room, m, out, None)
+    assert clip(m=-1.0) == INVALID and clip(m=float("nan")) == INVALID and clip(k=-1) == INVALID and clip(n=big, x=(ctypes.c_uint64 * 2)(1 << 30, 16), room=1) == LARGE
     assert clip(part=None) == NULL and clip(out=None) == NULL
     assert clip(x=(ctypes.c_uint64 * 2)(4096, 4096 + 396)) == OVERLAP and clip(x=(ctypes.c_uint64 * 2)(8192, 8192)) == OVERLAP
+    assert clip(x=(ctypes.c_uint64 * 2)(4096 + 396, 4096)) == OVERLAP
     assert lib.pinn_error_string(OVERLAP) == b"two tensors share memory"
 
 
@@ -170,9 +175,11 @@ def test_lists_of_tensors():
     ps[4].grad = torch.ones(9, 1).t()                                          # another stride of a dimension of one element: the same order
     assert gather() == (4, [2]) and g[2] == 0 and g[4] == ps[4].grad.data_ptr()
     before = [q._version for q in ps]
-    native.written(ps, C.addressof(count))
+    native.written(ps, False, C.addressof(count))
     assert [q._version - b for q, b in zip(ps, before)] == [1, 0, 1, 1, 1, 0]
-    assert [x.data_ptr() for x in native.grads(ps)] == [q.grad.data_ptr() for q in ps[:5]]
+    before = [q.grad._version for q in ps[:5]]
+    native.written(ps, True, 0)
+    assert [q.grad._version - b for q, b in zip(ps, before)] == [1] * 5
     dtype[3] = 1
     with pytest.raises(ValueError, match="parameter 3 is not what it was"):
         gather()
@@ -188,17 +195,25 @@ def test_lists_of_tensors():
     ps[0].grad = torch.sparse_coo_tensor(torch.tensor([[0], [1]]), torch.tensor([1.0]), (3, 5))
     with pytest.raises(ValueError, match="gradient of parameter 0"):
         gather()
-    x = (C.c_uint64 * 3)()
+    x = (C.c_uint64 * 6)()
 
-    def describe(ts):
-        return native.describe(ts, C.addressof(x), C.addressof(numel), C.addressof(dtype))
+    def describe(ts, of_grads=False):
+        return native.describe(ts, of_grads, C.addressof(x), C.addressof(numel), C.addressof(dtype))
     a = torch.randn(4, 6)
-    assert describe([a, a.t(), a[:, ::2]]) == [2] and list(x)[:2] == [a.data_ptr()] * 2 and list(numel)[:3] == [24, 24, 12]
-    for bad in (a.double(), a.long(), a.to_sparse()):
+    with pytest.raises(NativeError, match="no CPU fallback"):
+        describe([a])
+    a = torch.empty(4, 6, device="meta")                                       # no GPU here: what it reads beside the addresses
+    assert describe([a, a.t(), a[:, ::2], a[:0].bfloat16()]) == (4, [(2, 2)], -1)
+    assert list(numel)[:4] == [24, 24, 12, 0] and list(dtype)[:4] == [0, 0, 0, 1]
+    qs = [torch.nn.Parameter(t) for t in (a, a[0], a[1])]
+    assert describe(qs, True) == (0, [], None)
+    qs[1].grad, qs[2].grad = torch.empty(6, device="meta"), torch.empty(12, device="meta")[::2]
+    assert describe(qs, True) == (2, [(1, 2)], -1)
+    for bad in (a.double(), a.long(), torch.empty(4, 6, layout=torch.sparse_coo, device="meta")):
         with pytest.raises(ValueError, match="tensor 1"):
             describe([a, bad])
     with pytest.raises(ValueError, match="one device"):
-        describe([a, torch.empty(2, device="meta")])
-    for call in (lambda: describe([a, 3]), lambda: native.grads([a, None]), lambda: native.gather([None] * 6, 0, 0, 0, 0, 0), lambda: native.grads((a,)), lambda: describe((a,))):
+        describe([a, torch.empty(2)])
+    for call in (lambda: describe([a, 3]), lambda: native.gather([None] * 6, 0, 0, 0, 0, 0), lambda: describe((a,)), lambda: native.written([a, None], False, 0)):
         with pytest.raises(TypeError):
             call()

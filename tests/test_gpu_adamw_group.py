@@ -441,6 +441,10 @@ def test_grad_norm_of_mixed_many_strided_and_extreme():
     assert abs(float(grad_norm(small)) / (1e-30 * 3000 ** 0.5) - 1) < 1e-6
     assert torch.isnan(grad_norm([big, torch.tensor([float("nan")], device=cuda())]))
     assert float(grad_norm(torch.empty(0, device=cuda()))) == 0.0 and float(grad_norm([])) == 0.0
+    empty = params_of([torch.empty(0, device=cuda()) for _ in range(300)])
+    for p in empty:
+        p.grad = torch.empty(0, device=cuda())
+    assert float(grad_norm([p.grad for p in empty])) == 0.0 and float(clip_grad_norm_(empty, 1.0)) == 0.0
     assert float(grad_norm(torch.tensor(-3.0, device=cuda()))) == 3.0
 
 
@@ -471,10 +475,27 @@ def test_clip_grad_norm(max_norm):
             assert np.array_equal(f64(p.grad), g)
 
 
-def test_clip_grad_norm_of_norms_that_are_not_finite():
+@pytest.mark.parametrize("n_tensors,size", [(1, 1), (10, 785), (64, 256), (65, 252), (16, 1024), (17, 1024), (1, 16384), (1, 16385), (700, 3)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_clip_grad_norm_around_the_one_launch_form(dtype, n_tensors, size):
+    """few elements take one workgroup, 16384 elements and 64 tensors are its limits"""
+    params = params_of(make([(size,)] * n_tensors, dtype, 106))
+    for p, g in zip(params, make([(size,)] * n_tensors, dtype, 107, 2.0)):
+        p.grad = g
+    had = [f64(p.grad) for p in params]
+    norm, f = F.clip_factor(had, 0.5)
+    assert torch.equal(grad_norm([p.grad for p in params]), clip_grad_norm_(params, 1e9))
+    assert all(np.array_equal(f64(p.grad), g) for p, g in zip(params, had))
+    assert abs(float(clip_grad_norm_(params, 0.5)) - norm) <= 2 * H * norm
+    for p, g in zip(params, had):
+        assert (np.abs(f64(p.grad) - g * f) <= 2 * H * np.abs(g * f) + half_step(p.dtype, g * f)).all()
+
+
+@pytest.mark.parametrize("size", [1000, 20000])
+def test_clip_grad_norm_of_norms_that_are_not_finite(size):
     for bad in (float("nan"), float("inf")):
-        p = params_of(make([(1000,)], torch.float32, 110))[0]
-        p.grad = make([(1000,)], torch.float32, 111)[0]
+        p = params_of(make([(size,)], torch.float32, 110))[0]
+        p.grad = make([(size,)], torch.float32, 111)[0]
         p.grad[17] = bad
         before = p.grad.clone()
         with pytest.raises(RuntimeError, match="not clipped"):
