@@ -57,15 +57,16 @@ PyObject *guarded(F f)
     return nullptr;
 }
 
-// gather(params, numel, dtype, p, g, count) -> (gradients found, [indices whose gradient lies in another order than its parameter])
+// gather(params, numel, dtype, p, g, count) -> (gradients found, [indices whose gradient lies in another order than its parameter], whether
+// a parameter lies elsewhere than p said before)
 // numel, dtype: int64 and int32 arrays, what the plan was made for; p, g: uint64 arrays that take the addresses (g: 0 without a gradient);
-// count: int64 array, the gradient's length or 0.  Arrays are given by their address.
+// count: int64 array, the gradient's length or 0.  Arrays are given by their address.  The parameters that have a gradient count as written to.
 PyObject *gather(PyObject *, PyObject *args)
 {
     PyObject *params;
     unsigned long long a_numel, a_dtype, a_p, a_g, a_count;
     if (!PyArg_ParseTuple(args, "O!KKKKK", &PyList_Type, &params, &a_numel, &a_dtype, &a_p, &a_g, &a_count)) return nullptr;
-    return guarded([&]() -> PyObject * {
+    const auto found = guarded([&]() -> PyObject * {
         const int64_t *numel = (const int64_t *)(uintptr_t)a_numel;
         const int32_t *dtype = (const int32_t *)(uintptr_t)a_dtype;
         uint64_t *p_out = (uint64_t *)(uintptr_t)a_p, *g_out = (uint64_t *)(uintptr_t)a_g;
@@ -74,6 +75,7 @@ PyObject *gather(PyObject *, PyObject *args)
         PyObject *other = PyList_New(0);
         if (!other) return nullptr;
         Py_ssize_t given = 0;
+        bool moved = false;
         c10::Device device(c10::DeviceType::CPU);
         for (Py_ssize_t i = 0; i < n; ++i) {
             if (!tensor_at(params, i, "parameter")) { Py_DECREF(other); return nullptr; }
@@ -84,7 +86,9 @@ PyObject *gather(PyObject *, PyObject *args)
                 Py_DECREF(other);
                 return nullptr;
             }
-            p_out[i] = (uint64_t)(uintptr_t)p.data_ptr();
+            const uint64_t at = (uint64_t)(uintptr_t)p.data_ptr();
+            moved |= p_out[i] != at;
+            p_out[i] = at;
             g_out[i] = 0;
             count[i] = 0;
             const at::Tensor &g = p.grad();
@@ -106,8 +110,15 @@ PyObject *gather(PyObject *, PyObject *args)
                 if (bad) { Py_DECREF(other); return nullptr; }
             }
         }
-        return Py_BuildValue("(nN)", given, other);
+        for (Py_ssize_t i = 0; i < n; ++i)
+            if (count[i]) {
+                const at::Tensor &p = THPVariable_Unpack(PyList_GET_ITEM(params, i));
+                if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+            }
+        return Py_BuildValue("(nNO)", given, other, moved ? Py_True : Py_False);
     });
+    if (!found && a_p && PyList_GET_SIZE(params) > 0) *(uint64_t *)(uintptr_t)a_p = 0;   // the next call says "moved" again
+    return found;
 }
 
 // describe(tensors, of_grads, x, numel, dtype) -> (how many, [(place in the arrays, index) of those that are neither contiguous nor another
@@ -167,22 +178,18 @@ PyObject *describe(PyObject *, PyObject *args)
     });
 }
 
-// written(tensors, of_grads, which): the tensors (or their gradients) were written to in place; which: int64 array, 0 leaves one out, or
-// no array
-PyObject *written(PyObject *, PyObject *args)
+// grads_written(params): the gradients of those that have one were written to in place
+PyObject *grads_written(PyObject *, PyObject *list)
 {
-    PyObject *list;
-    int of_grads;
-    unsigned long long a_which;
-    if (!PyArg_ParseTuple(args, "O!pK", &PyList_Type, &list, &of_grads, &a_which)) return nullptr;
+    if (!PyList_Check(list)) {
+        PyErr_SetString(PyExc_TypeError, "a list is needed");
+        return nullptr;
+    }
     return guarded([&]() -> PyObject * {
-        const int64_t *which = (const int64_t *)(uintptr_t)a_which;
         for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-            if (which && !which[i]) continue;
-            if (!tensor_at(list, i, "tensor")) return nullptr;
-            const at::Tensor &given = THPVariable_Unpack(PyList_GET_ITEM(list, i));
-            const at::Tensor &t = of_grads ? given.grad() : given;
-            if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+            if (!tensor_at(list, i, "parameter")) return nullptr;
+            const at::Tensor &g = THPVariable_Unpack(PyList_GET_ITEM(list, i)).grad();
+            if (g.defined() && !g.is_inference()) g.unsafeGetTensorImpl()->bump_version();
         }
         Py_RETURN_NONE;
     });
@@ -190,7 +197,7 @@ PyObject *written(PyObject *, PyObject *args)
 
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, nullptr},
                          {"describe", describe, METH_VARARGS, nullptr},
-                         {"written", written, METH_VARARGS, nullptr},
+                         {"grads_written", grads_written, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -215,7 +215,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
         _check(rc, "pinn_grad_clip")
         for g, c in lst.back:
             g.copy_(c)
-    load_tensorlist().written(parameters, True, 0)
+    load_tensorlist().grads_written(parameters)
     return norm
 
 
@@ -330,14 +330,15 @@ class GroupedAdamW(torch.optim.Optimizer):
             first += len(rows)
 
     def _launch(self, grp, dtype, rows, first):
-        parts, chunk = [np.zeros(0, dtype=ADAMW_CHUNK_DTYPE)], ADAMW_CHUNK32 if self.state_bits == 32 else ADAMW_CHUNK8
-        for k, i in enumerate(rows):
-            base = np.arange(0, self._params[i].numel(), chunk, dtype=np.int64)
-            part = np.zeros(len(base), dtype=ADAMW_CHUNK_DTYPE)
-            part["base"], part["place"], part["tensor"], part["row"] = base, self.offsets[i] + base, k, i
-            part["count"] = np.minimum(self._params[i].numel() - base, chunk)
-            parts.append(part)
-        parts = np.concatenate(parts)
+        chunk = ADAMW_CHUNK32 if self.state_bits == 32 else ADAMW_CHUNK8
+        numel = np.array([self._params[i].numel() for i in rows], dtype=np.int64)
+        count = -(-numel // chunk)
+        k = np.repeat(np.arange(len(rows)), count)
+        parts = np.zeros(len(k), dtype=ADAMW_CHUNK_DTYPE)
+        parts["base"] = (np.arange(len(k)) - (np.cumsum(count) - count)[k]) * chunk
+        parts["place"] = np.array([self.offsets[i] for i in rows], dtype=np.int64)[k] + parts["base"]
+        parts["count"] = np.minimum(numel[k] - parts["base"], chunk)
+        parts["tensor"], parts["row"] = k, np.array(rows)[k]
         chunks = torch.from_numpy(parts.view(np.uint8)).to(self.device)
         where = torch.tensor(rows, dtype=torch.int32, device=self.device)
         d = PinnAdamWGroup()
@@ -427,7 +428,11 @@ class GroupedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         hyper = {id(grp): self._hyper(grp) for grp in self.param_groups}
-        given, other = self._native.gather(self._ordered, *self._gather_args)
+        given, other, moved = self._native.gather(self._ordered, *self._gather_args)
+        if moved:
+            self._p[0], first = 0, self._p[0]           # found wanting, they are looked at again in the next step
+            self._check_params()
+            self._p[0] = first
         if not given:
             return loss
         keep = []
@@ -450,7 +455,6 @@ class GroupedAdamW(torch.optim.Optimizer):
                 d.partials, d.n_partials = partials.data_ptr() if n_partials else None, n_partials
                 d.max_norm, d.skip_nonfinite = -1.0 if self.max_norm is None else self.max_norm, self.skip_nonfinite
                 _check(self.lib.pinn_adamw_group_step(launch["ref"], launch["p"], launch["g"], stream), "pinn_adamw_group_step")
-        self._native.written(self._ordered, False, self._gather_args[4])
         return loss
 
     _hooked_step = torch.optim.Optimizer.profile_hook_step(_step)

@@ -166,19 +166,18 @@ def test_lists_of_tensors():
 
     def gather():
         return native.gather(ps, *(C.addressof(x) for x in (numel, dtype, p, g, count)))
-    assert gather() == (0, []) and list(g) == [0] * n and list(count) == [0] * n
+    assert gather() == (0, [], True) and list(g) == [0] * n and list(count) == [0] * n
     for q in ps[:5]:
         q.grad = torch.ones_like(q)
-    assert gather() == (4, []) and list(count) == [15, 0, 28, 6, 9, 0]
+    before = [q._version for q in ps]
+    assert gather() == (4, [], False) and list(count) == [15, 0, 28, 6, 9, 0]
     assert list(p) == [q.data_ptr() for q in ps] and g[0] == ps[0].grad.data_ptr() and g[1] == g[5] == 0
     ps[2].grad = torch.ones(4, 7)                                              # another order than its parameter's
     ps[4].grad = torch.ones(9, 1).t()                                          # another stride of a dimension of one element: the same order
-    assert gather() == (4, [2]) and g[2] == 0 and g[4] == ps[4].grad.data_ptr()
-    before = [q._version for q in ps]
-    native.written(ps, False, C.addressof(count))
-    assert [q._version - b for q, b in zip(ps, before)] == [1, 0, 1, 1, 1, 0]
+    assert gather() == (4, [2], False) and g[2] == 0 and g[4] == ps[4].grad.data_ptr()
+    assert [q._version - b for q, b in zip(ps, before)] == [2, 0, 2, 2, 2, 0]
     before = [q.grad._version for q in ps[:5]]
-    native.written(ps, True, 0)
+    native.grads_written(ps)
     assert [q.grad._version - b for q, b in zip(ps, before)] == [1] * 5
     dtype[3] = 1
     with pytest.raises(ValueError, match="parameter 3 is not what it was"):
@@ -187,7 +186,9 @@ def test_lists_of_tensors():
     ps[0].data = torch.randn(3, 6)
     with pytest.raises(ValueError, match="parameter 0"):
         gather()
+    assert p[0] == 0                                                           # so that the next call says "moved"
     ps[0].data = torch.randn(3, 5)
+    assert gather() == (4, [2], True) and gather() == (4, [2], False)
     ps[0].grad.data = torch.ones(5, 3)
     with pytest.raises(ValueError, match="gradient of parameter 0"):
         gather()
@@ -214,6 +215,6 @@ def test_lists_of_tensors():
             describe([a, bad])
     with pytest.raises(ValueError, match="one device"):
         describe([a, torch.empty(2)])
-    for call in (lambda: describe([a, 3]), lambda: native.gather([None] * 6, 0, 0, 0, 0, 0), lambda: describe((a,)), lambda: native.written([a, None], False, 0)):
+    for call in (lambda: describe([a, 3]), lambda: native.gather([None] * 6, 0, 0, 0, 0, 0), lambda: describe((a,)), lambda: native.grads_written([a, None]), lambda: native.grads_written((a,))):
         with pytest.raises(TypeError):
             call()

@@ -415,6 +415,52 @@ def test_agrees_with_the_flat_step():
         assert ((a - b).abs() <= 20 * 48 * H * (a.abs() + 1e-2)).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipping_before_the_step_is_clipping_inside_it(bits):
+    """as they are used together: clip_grad_norm_ then step, against max_norm.  The clipped gradient is rounded to float32 once more (h of m and
+    2 h of v, so at most 3 h of the update), in 8 bits a code may then fall on the other side: the weights alone are compared there, over one step"""
+    n_steps = 4 if bits == 32 else 1
+    a, b = params_of(make(SIZES, torch.float32, 85)), params_of(make(SIZES, torch.float32, 85))
+    oa, ob = GroupedAdamW(a, state_bits=bits, **HYPER), GroupedAdamW(b, state_bits=bits, max_norm=0.5, **HYPER)
+    for k in range(n_steps):
+        for p, q, g in zip(a, b, make(SIZES, torch.float32, 86 + k)):
+            p.grad, q.grad = g.clone(), g
+        norm = clip_grad_norm_(a, 0.5)
+        oa.step()
+        ob.step()
+        assert abs(float(norm) / float(ob.grad_norm) - 1) <= 2 * H
+    for p, q in zip(a, b):
+        assert ((p - q).abs() <= n_steps * (4 * H * q.abs() + 24 * H * HYPER["lr"] * 10)).all()   # |U| <= 10 lr, generously: |m| / sqrt(v) hat is near 1
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.float32, 32), (torch.bfloat16, 8)])
+def test_a_tensor_beyond_32_bits(dtype, bits):
+    """2^31 + 4999 elements: offsets in bytes and in elements pass 32 bits; three places are held to the formula, and the norm to the sum of a constant"""
+    n = (1 << 31) + 4999
+    p = torch.nn.Parameter(torch.full((n,), 0.25, dtype=dtype, device=cuda()))
+    p.grad = torch.full((n,), 2.0 ** -10, dtype=dtype, device=cuda())
+    opt = GroupedAdamW([p], state_bits=bits, max_norm=1.0, **HYPER)
+    places = [slice(0, 1024), slice((1 << 31) - 512, (1 << 31) + 512), slice(n - 3079, n)]
+    rng = np.random.default_rng(0)
+    for s in places:
+        p.grad[s] = torch.tensor(rng.standard_normal(s.stop - s.start) * 2.0 ** -10, device=cuda()).to(dtype)
+    grads = [f64(p.grad[s]) for s in places]
+    rest = n - sum(s.stop - s.start for s in places)
+    norm = np.sqrt(sum((g ** 2).sum() for g in grads) + rest * 2.0 ** -20)
+    opt.step()
+    assert abs(float(opt.grad_norm) / norm - 1) <= 2 * H
+    ms, vs = (x[:n] for x in opt.moments())
+    for s, g in zip(places, grads):
+        p1, m1, v1 = F.step(np.full(len(g), 0.25), g * (1.0 / (norm + 1e-6)), 0.0, 0.0, 1, HYPER["lr"], 0.9, 0.999, 1e-8, HYPER["weight_decay"])
+        # |U| is at most lr / (1 - b1) (1 - b1) / sqrt((1 - b2) / (1 - b2)) = lr at the first step
+        assert (np.abs(f64(p[s]) - p1) <= H * (3 * 0.26 + 24 * HYPER["lr"]) + half_step(dtype, p1)).all()
+        if bits == 32:
+            assert (np.abs(f64(ms[s]) - m1) <= 5 * H * np.abs(m1)).all() and (np.abs(f64(vs[s]) - v1) <= 8 * H * v1).all()
+        else:
+            assert s.start % F.BLOCK == 0 and (s.stop % F.BLOCK == 0 or s.stop == n)
+            assert np.array_equal(f64(ms[s]), F.round_flat(m1, s.start, 1, F.M)[0]) and np.array_equal(f64(vs[s]), F.round_flat(v1, s.start, 1, F.V)[0])
+
+
 # ---- the norm ----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_grad_norm(dtype):
@@ -535,6 +581,14 @@ def test_refusals():
         GroupedAdamW([torch.nn.Parameter(base[::2])])
     with pytest.raises(ValueError, match="float64"):
         GroupedAdamW([torch.nn.Parameter(base.double())])
+    with pytest.raises(ValueError, match="share memory"):
+        tied = params_of(make([(50,), (50,)], torch.float32, 122))
+        opt = GroupedAdamW(tied)
+        tied[1].data = tied[0].data                                            # tied only later
+        tied[0].grad = torch.ones(50, device=cuda())
+        with pytest.raises(ValueError, match="share memory"):
+            opt.step()
+        opt.step()
     opt = GroupedAdamW([torch.nn.Parameter(base)])
     with pytest.raises(ValueError, match="all parameter groups"):
         opt.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(2, device=cuda()))]))
