@@ -437,20 +437,22 @@ __global__ __launch_bounds__(kThreads, BITS == 32 ? 6 : 5) void k_adamw_group(co
     // The workgroup that finishes last advances the counters: every other one has used what it read of them by then.  Nothing
     // else passes between workgroups, so the tickets need no fence (a device-wide one writes the caches back, once per workgroup).
     // Atomics on one word take 11 ns each, one after the other (2048 of them 23 us, a third of a step of 5M weights): a
-    // workgroup draws from one of kTickets words on lines of their own, and the last of those draws from the first word.
+    // workgroup of a large grid draws from one of kTickets words on lines of their own, and the last of those draws from the first word.
     __shared__ bool last_of_all;
     __syncthreads();
     if (threadIdx.x == 0) {
-        const unsigned groups = gridDim.x < kTickets ? gridDim.x : kTickets, j = blockIdx.x % kTickets;
-        uint32_t *mine = c.ticket + (1 + j) * kTicketStride;
-        last_of_all = false;
-        if (draw(mine) == (gridDim.x - j + kTickets - 1) / kTickets - 1) {
-            put_back(mine);
-            if (draw(c.ticket) == groups - 1) {
-                put_back(c.ticket);
-                last_of_all = true;
+        if (gridDim.x <= kTickets) {
+            last_of_all = draw(c.ticket) == gridDim.x - 1;
+        } else {
+            const unsigned j = blockIdx.x % kTickets;
+            uint32_t *mine = c.ticket + (1 + j) * kTicketStride;
+            last_of_all = false;
+            if (draw(mine) == (gridDim.x - j + kTickets - 1) / kTickets - 1) {
+                put_back(mine);
+                last_of_all = draw(c.ticket) == kTickets - 1;
             }
         }
+        if (last_of_all) put_back(c.ticket);
     }
     __syncthreads();
     if (!last_of_all) return;
@@ -603,8 +605,8 @@ __global__ __launch_bounds__(kThreads) void k_grad_clip(const NormArgs a, const 
 
 // Few elements: ONE workgroup forms the norm and, with max_norm >= 0, scales, a wave to a tensor at a time.  A launch is 3.7 us at the
 // host, so for a small net the second one is a third of the call.
-constexpr int kSmallThreads = 1024, kSmallTensors = 64;
-constexpr int64_t kSmallElements = 16384;
+constexpr int kSmallThreads = 1024, kSmallTensors = PINN_NORM_SMALL_TENSORS;
+constexpr int64_t kSmallElements = PINN_NORM_SMALL_ELEMENTS;
 
 template <class T, class F>
 __device__ inline void wave_over(T *x, int n, F f)
@@ -724,12 +726,11 @@ bool small_list(NormArgs &a, void *const *x, const int64_t *numel, const int32_t
 {
     int64_t total = 0;
     for (int i = 0; i < n; ++i) {
-        total += numel[i] < kSmallElements ? numel[i] : kSmallElements + 1;
+        total += numel[i] <= kSmallElements ? numel[i] : kSmallElements + 1;
         if (total > kSmallElements) return false;
     }
     NormPlan plan;
-    plan.advance(a, x, numel, dtype, n);
-    return plan.next == n && a.n_tensors <= kSmallTensors;
+    return n <= kSmallTensors && (plan.advance(a, x, numel, dtype, n), true);
 }
 
 int launch_sumsq(const void *const *grads, const int64_t *numel, const int32_t *dtype, int n_tensors, double *partials, int64_t n_reserved,
@@ -772,12 +773,13 @@ extern "C" int pinn_grad_norm(const void *const *grads, const int64_t *numel, co
                               int64_t n_reserved, float *norm, void *stream)
 {
     if (const int rc = check_list(grads, numel, dtype, n_tensors)) return rc;
-    if (!norm || !partials) return PINN_ERR_NULL;
+    if (!norm) return PINN_ERR_NULL;
     NormArgs a;
     if (small_list(a, (void *const *)grads, numel, dtype, n_tensors)) {
         hipLaunchKernelGGL(k_norm_small, dim3(1), dim3(kSmallThreads), 0, (hipStream_t)stream, a, -1.0, norm);
         return launch_error();
     }
+    if (!partials) return PINN_ERR_NULL;
     int32_t n_partials = 0;
     if (const int rc = launch_sumsq(grads, numel, dtype, n_tensors, partials, n_reserved, &n_partials, stream)) return rc;
     hipLaunchKernelGGL(k_norm_of, dim3(1), dim3(kThreads), 0, (hipStream_t)stream, partials, (int)n_partials, norm);
@@ -788,7 +790,7 @@ extern "C" int pinn_grad_clip(void *const *grads, const int64_t *numel, const in
                               int64_t n_reserved, double max_norm, float *norm, void *stream)
 {
     if (const int rc = check_list((const void *const *)grads, numel, dtype, n_tensors)) return rc;
-    if (!norm || !partials) return PINN_ERR_NULL;
+    if (!norm) return PINN_ERR_NULL;
     if (!(max_norm >= 0.0)) return PINN_ERR_INVALID_DESC;
     if (const int rc = check_apart(grads, numel, dtype, n_tensors)) return rc;
     NormArgs a;
@@ -796,6 +798,7 @@ extern "C" int pinn_grad_clip(void *const *grads, const int64_t *numel, const in
         hipLaunchKernelGGL(k_norm_small, dim3(1), dim3(kSmallThreads), 0, (hipStream_t)stream, a, max_norm, norm);
         return launch_error();
     }
+    if (!partials) return PINN_ERR_NULL;
     int32_t n_partials = 0;
     if (const int rc = launch_sumsq((const void *const *)grads, numel, dtype, n_tensors, partials, n_reserved, &n_partials, stream)) return rc;
     NormPlan plan;

@@ -122,7 +122,7 @@ PyObject *gather(PyObject *, PyObject *args)
 }
 
 // describe(tensors, of_grads, x, numel, dtype) -> (how many, [(place in the arrays, index) of those that are neither contiguous nor another
-// order of the same memory], index of their GPU); of_grads: the gradients of those tensors that have one
+// order of the same memory], index of their GPU, elements in all); of_grads: the gradients of those tensors that have one
 PyObject *describe(PyObject *, PyObject *args)
 {
     PyObject *list;
@@ -138,6 +138,7 @@ PyObject *describe(PyObject *, PyObject *args)
         if (!other) return nullptr;
         c10::Device device(c10::DeviceType::CPU);
         Py_ssize_t k = 0;
+        int64_t total = 0;
         for (Py_ssize_t i = 0; i < n; ++i) {
             if (!tensor_at(list, i, "tensor")) { Py_DECREF(other); return nullptr; }
             const at::Tensor &given = THPVariable_Unpack(PyList_GET_ITEM(list, i));
@@ -164,6 +165,7 @@ PyObject *describe(PyObject *, PyObject *args)
             }
             x[k] = t.numel() ? (uint64_t)(uintptr_t)t.data_ptr() : 0;
             numel[k] = t.numel();
+            total += t.numel();
             dtype[k] = code_of(t);
             if (!dense(t)) {
                 PyObject *pair = Py_BuildValue("(nn)", k, i);
@@ -173,8 +175,8 @@ PyObject *describe(PyObject *, PyObject *args)
             }
             ++k;
         }
-        if (k == 0) return Py_BuildValue("(nNO)", k, other, Py_None);
-        return Py_BuildValue("(nNn)", k, other, (Py_ssize_t)device.index());
+        if (k == 0) return Py_BuildValue("(nNOi)", k, other, Py_None, 0);
+        return Py_BuildValue("(nNnL)", k, other, (Py_ssize_t)device.index(), (long long)total);
     });
 }
 

@@ -17,8 +17,9 @@ import numpy as np
 import torch
 import torch.optim.optimizer as _hooks
 
-from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, DTYPE_CODES, ERR_OVERLAP, NativeError, PinnAdamWGroup, _check, _cur_stream, _on, load_library,
-                      load_tensorlist)
+from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, DTYPE_CODES,
+                      ERR_OVERLAP, NORM_SMALL_ELEMENTS, NORM_SMALL_TENSORS, NativeError, PinnAdamWGroup, _check, _cur_stream, _on,
+                      load_library, load_tensorlist)
 
 
 class FusedAdam(torch.optim.Optimizer):
@@ -151,17 +152,23 @@ class _TensorList:
         n = len(tensors)
         self.x, self.numel, self.dtype = (ctypes.c_uint64 * n)(), (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
         at = ctypes.addressof(self.x), ctypes.addressof(self.numel), ctypes.addressof(self.dtype)
-        self.n, other, index = load_tensorlist().describe(tensors, of_grads, *at)
+        self.n, other, index, total = load_tensorlist().describe(tensors, of_grads, *at)
         self.device = None if index is None else torch.device("cuda", index)
         self.back = []
         for k, i in other:
             t = tensors[i].grad.detach() if of_grads else tensors[i].detach()
             self.back.append((t, t.contiguous()))
             self.x[k] = self.back[-1][1].data_ptr()
+        self.partials = None                            # the call's own workspace
+        if index is not None and (self.n > NORM_SMALL_TENSORS or total > NORM_SMALL_ELEMENTS):
+            self.partials, room = _partials(self.n, self.device)
+            self.args = self.x, self.numel, self.dtype, self.n, self.partials.data_ptr(), room
+        else:
+            self.args = self.x, self.numel, self.dtype, self.n, None, 0
 
 
 def _partials(n, device):
-    """(workspace of the call's own, its length)"""
+    """(room for partial sums, its length)"""
     room = load_library().pinn_grad_norm_partials(n)
     return torch.empty(room, dtype=torch.float64, device=device), room
 
@@ -179,10 +186,8 @@ def grad_norm(tensors):
         return torch.tensor(0.0)
     lst = _TensorList(tensors)
     norm = torch.empty((), dtype=torch.float32, device=lst.device)
-    partials, room = _partials(lst.n, lst.device)
     with _on(lst.device):
-        _check(load_library().pinn_grad_norm(lst.x, lst.numel, lst.dtype, lst.n, partials.data_ptr(), room, norm.data_ptr(), _cur_stream(norm)),
-               "pinn_grad_norm")
+        _check(load_library().pinn_grad_norm(*lst.args, norm.data_ptr(), _cur_stream(norm)), "pinn_grad_norm")
     return norm
 
 
@@ -201,15 +206,14 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     if any(0 in (st for sz, st in zip(g.shape, g.stride()) if sz > 1) for g, _ in lst.back):
         raise ValueError("a gradient that was expanded cannot be scaled in place")
     norm = torch.empty((), dtype=torch.float32, device=lst.device)
-    partials, room = _partials(lst.n, lst.device)
-    lib, args = load_library(), (lst.x, lst.numel, lst.dtype, lst.n, partials.data_ptr(), room)
+    lib = load_library()
     with _on(lst.device):
         stream = _cur_stream(norm)
         if error_if_nonfinite:
-            _check(lib.pinn_grad_norm(*args, norm.data_ptr(), stream), "pinn_grad_norm")
+            _check(lib.pinn_grad_norm(*lst.args, norm.data_ptr(), stream), "pinn_grad_norm")
             if not torch.isfinite(norm):
                 raise RuntimeError("the gradients' norm is %s: they were not clipped" % norm.item())
-        rc = lib.pinn_grad_clip(*args, max_norm, norm.data_ptr(), stream)
+        rc = lib.pinn_grad_clip(*lst.args, max_norm, norm.data_ptr(), stream)
         if rc == ERR_OVERLAP:
             raise ValueError("two of the gradients share memory: scaling them in place would scale it twice")
         _check(rc, "pinn_grad_clip")

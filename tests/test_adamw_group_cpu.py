@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import adamw_formulas as F
-from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, NativeError, PinnAdamWGroup, load_library
+from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, NORM_SMALL_ELEMENTS, NORM_SMALL_TENSORS, NativeError, PinnAdamWGroup, load_library
 from pde_amd.optim import GroupedAdamW, clip_grad_norm_, grad_norm
 from conftest import GOLDEN, ROOT
 
@@ -79,7 +79,8 @@ def test_c_entries_refuse_without_a_gpu():
     lib = load_library()
     header = open(os.path.join(ROOT, "include", "pinnjet.h")).read()
     for name, value in (("PINN_ADAMW_BLOCK", ADAMW_BLOCK), ("PINN_ADAMW_CHUNK32", ADAMW_CHUNK32), ("PINN_ADAMW_CHUNK8", ADAMW_CHUNK8), ("PINN_ADAMW_MAX_TENSORS", ADAMW_MAX_TENSORS),
-                        ("PINN_ADAMW_TICKET_WORDS", ADAMW_TICKET_WORDS)):
+                        ("PINN_ADAMW_TICKET_WORDS", ADAMW_TICKET_WORDS), ("PINN_NORM_SMALL_TENSORS", NORM_SMALL_TENSORS),
+                        ("PINN_NORM_SMALL_ELEMENTS", NORM_SMALL_ELEMENTS)):
         assert "#define %s %d " % (name, value) in header
     assert ADAMW_CHUNK_DTYPE.itemsize == 32 and ctypes.sizeof(PinnAdamWGroup) == 168
     one = (ctypes.c_uint64 * 2)(4096, 8192)
@@ -125,12 +126,12 @@ def test_c_entries_refuse_without_a_gpu():
     def norm(x=one, n=n2, dt=f32, k=2, part=16, room=4096, out=16):
         return lib.pinn_grad_norm(x, n, dt, k, part, room, out, None)
     big = (ctypes.c_int64 * 2)(1 << 20, 100)
-    assert norm(part=None) == NULL and norm(out=None) == NULL and norm(x=None) == NULL and norm(k=-1) == INVALID and norm(n=big, room=1) == LARGE
+    assert norm(part=None, n=big) == NULL and norm(out=None) == NULL and norm(x=None) == NULL and norm(k=-1) == INVALID and norm(n=big, room=1) == LARGE
 
     def clip(x=one, n=n2, k=2, part=16, m=1.0, out=16, room=4096):
         return lib.pinn_grad_clip(x, n, f32, k, part, room, m, out, None)
     assert clip(m=-1.0) == INVALID and clip(m=float("nan")) == INVALID and clip(k=-1) == INVALID and clip(n=big, x=(ctypes.c_uint64 * 2)(1 << 30, 16), room=1) == LARGE
-    assert clip(part=None) == NULL and clip(out=None) == NULL
+    assert clip(part=None, n=big, x=(ctypes.c_uint64 * 2)(1 << 30, 16)) == NULL and clip(out=None) == NULL
     assert clip(x=(ctypes.c_uint64 * 2)(4096, 4096 + 396)) == OVERLAP and clip(x=(ctypes.c_uint64 * 2)(8192, 8192)) == OVERLAP
     assert clip(x=(ctypes.c_uint64 * 2)(4096 + 396, 4096)) == OVERLAP
     assert lib.pinn_error_string(OVERLAP) == b"two tensors share memory"
@@ -204,12 +205,12 @@ def test_lists_of_tensors():
     with pytest.raises(NativeError, match="no CPU fallback"):
         describe([a])
     a = torch.empty(4, 6, device="meta")                                       # no GPU here: what it reads beside the addresses
-    assert describe([a, a.t(), a[:, ::2], a[:0].bfloat16()]) == (4, [(2, 2)], -1)
+    assert describe([a, a.t(), a[:, ::2], a[:0].bfloat16()]) == (4, [(2, 2)], -1, 60)
     assert list(numel)[:4] == [24, 24, 12, 0] and list(dtype)[:4] == [0, 0, 0, 1]
     qs = [torch.nn.Parameter(t) for t in (a, a[0], a[1])]
-    assert describe(qs, True) == (0, [], None)
+    assert describe(qs, True) == (0, [], None, 0)
     qs[1].grad, qs[2].grad = torch.empty(6, device="meta"), torch.empty(12, device="meta")[::2]
-    assert describe(qs, True) == (2, [(1, 2)], -1)
+    assert describe(qs, True) == (2, [(1, 2)], -1, 12)
     for bad in (a.double(), a.long(), torch.empty(4, 6, layout=torch.sparse_coo, device="meta")):
         with pytest.raises(ValueError, match="tensor 1"):
             describe([a, bad])
