@@ -4,7 +4,8 @@
 //   m <- b1 m + (1 - b1) f g,   v <- b2 v + (1 - b2) (f g)^2
 //   p <- (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// Every element is read and written once (28 bytes for float32 throughout), so the step is bound by memory.  The tensors
+// Every element is read and written once (28 bytes for float32 throughout), so the step is bound by memory: 240M float32 weights
+// 1.08 ms (6.2 TB/s; a copy of 4 GB by torch runs at 4.7), clipped 1.21 ms with the gradient read twice.  The tensors
 // are cut into chunks of 1024 or 2048 elements; a table that the caller keeps on the device says which tensor a chunk lies in, so
 // one launch covers up to kMaxTensors tensors of any sizes; their addresses travel in the launch's arguments, because
 // gradients move from step to step.  Moments and master weights are flat buffers in which each tensor starts at a multiple of kBlock.
@@ -14,9 +15,11 @@
 // Scales are powers of two, so decoding and scaling are exact and the only rounding is the one to the byte.  It rounds up
 // with probability equal to the remainder, by a sequence over steps and elements that covers [0, 1) evenly:
 // with b2 = 0.999 a moment changes by less than half a code per step, and rounding to nearest would freeze it.
-// The arithmetic is float64 (as fast as unpacked float32 on this hardware): the top 20 bits of a double's mantissa hold the
-// 3 bits of the code and 17 bits of remainder, so rounding is one integer addition on the double's upper word, and it is exact -
-// the codes do not depend on how a compiler contracts a float32 expression.
+// The arithmetic is float64, whose products, sums and conversions issue as fast as integer operations here (4.4 to 5.4 cycles a
+// wave; float32 additions 2.8): the top 20 bits of a double's mantissa hold the 3 bits of the code and 17 bits of remainder, so
+// rounding is one integer addition on the double's upper word, and it is exact - the codes do not depend on how a compiler
+// contracts a float32 expression.  240M weights: float32 652 us (16 bytes each, 5.9 TB/s), bfloat16 430 us (10 bytes, 5.6 TB/s: its 48
+// vector instructions an element, 335 us of issue, no longer hide under 387 us of memory).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>
@@ -248,10 +251,22 @@ __device__ inline int scale_of(uint32_t hi, const Format &f)
     return s < 0 ? 0 : s > f.most_scale ? f.most_scale : s;
 }
 
-// x's magnitude as a code before it is held to the largest: 3 ldexp'd mantissa bits and what the remainder adds
-__device__ inline uint32_t code_of(double x, int exponent, uint32_t w)
+// x's magnitude as a code before it is held to the largest: 3 mantissa bits and what the remainder adds to them.  The place y on the
+// codes' scale (8 times the exponent field plus 8 times the fraction) is a float64 too: where its 53 bits end above x's last ones they are rounded,
+// and a y that is so rounded up to the next 2^-17 carries into the sum.  NEAR does that; without it `low` collects x's lower word, which
+// says whether any x is near enough (8 or fewer units below) for it to matter.
+template <bool NEAR>
+__device__ inline uint32_t code_of(double x, int exponent, uint32_t w, uint32_t &low)
 {
-    const uint32_t hi = (uint32_t)__double2hiint(ldexp(fabs(x), exponent));
+    const double scaled = ldexp(fabs(x), exponent);
+    uint32_t hi = (uint32_t)__double2hiint(scaled);
+    const uint32_t lo = (uint32_t)__double2loint(scaled);
+    if constexpr (NEAR) {
+        const uint32_t e = hi >> 20, half = e >= 16 ? 8u : e >= 8 ? 4u : e >= 4 ? 2u : e >= 2 ? 1u : 0u;   // half a unit of y's last place, in units of x's
+        if (half && lo >= 0u - half) ++hi;
+    } else {
+        low = lo > low ? lo : low;
+    }
     return (hi + (w >> 15 | 1u)) >> 17;
 }
 
@@ -262,6 +277,16 @@ struct Hyper8 {
     double b1, b2, g1, g2;                      // g1 = (1 - b1) f, g2 = (1 - b2) f^2
     float eps, decay;
 };
+
+// a b + c d with each operation rounded by itself.  Codes are compared with where the remainder lies, and (9 m + g) / 10 lies on such a
+// border more often than chance: m has 4 bits and g 24.  Which way 0.9 m + 0.1 g falls there is a matter of float64's last
+// bit, so the order of rounding is fixed: with fma, one or two codes in 5M differ from what the formula gives step by step.
+__device__ inline double product_sum(double a, double b, double c, double d)
+{
+#pragma clang fp contract(off)
+    const double x = a * b, y = c * d;
+    return x + y;
+}
 
 // A lane's 8 elements of a block: two runs of 4, APART elements from each other.  16-bit weights without masters: one run of 8
 // (16 bytes).  With float32 among them the runs are half a block apart, so that 16 lanes read 256 bytes in a row and not every
@@ -280,6 +305,28 @@ __device__ inline void store_runs(T *p, Vec<T, 8> x, int have)
     if constexpr (APART == 4) return store_some<FULL, 8>(p, x, have);
     store_some<FULL, 4>(p, __builtin_shufflevector(x, x, 0, 1, 2, 3), have);
     store_some<FULL, 4>(p + APART, __builtin_shufflevector(x, x, 4, 5, 6, 7), have - APART);
+}
+
+// behind the tensor's end gradients and codes are zero, and so are the codes that come out
+template <bool NEAR, int APART>
+__device__ inline void encode(const double (&md)[8], const double (&vd)[8], int xm, int xv, uint32_t w0m, uint32_t w0v, Vec<uint32_t, 2> &om,
+                              Vec<uint32_t, 2> &ov, uint32_t &low)
+{
+    om = 0;
+    ov = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t off = e < 4 ? e : APART + e - 4;
+        uint32_t a = code_of<NEAR>(md[e], xm, w0m + off * kPlaceM, low), b = code_of<NEAR>(vd[e], xv, w0v + off * kPlaceV, low);
+        a = a > kM.most_code ? kM.most_code : a;
+        a |= (uint32_t)__double2hiint(md[e]) >> 24 & 128u;
+        // 1 where v is not zero (written out: as a comparison it takes twice the instructions): a v that vanished under a live m would divide it by eps alone
+        uint32_t live;
+        asm("v_min_u32 %0, 1, %1" : "=v"(live) : "v"(__double2hiint(vd[e])));
+        asm("v_med3_u32 %0, %1, %2, %3" : "=v"(b) : "v"(b), "v"(live), "s"(kV.most_code));
+        om[e / 4] |= a << (8 * (e & 3));
+        ov[e / 4] |= b << (8 * (e & 3));
+    }
 }
 
 template <bool FULL, bool MASTER, class T>
@@ -319,8 +366,8 @@ __device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper8 &h)
         const float fm = (e & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(pair, true) : __builtin_amdgcn_cvt_pk_f32_fp8(pair, false))[e & 1];
         const float fv = __uint_as_float((e & 3) == 3 ? cv[e / 4] >> 4 & 0x0ff00000u : cv[e / 4] << (20 - 8 * (e & 3)) & 0x0ff00000u);
         const double gd = (double)(float)g[e];
-        md[e] = fma((double)fm, um, h.g1 * gd);
-        vd[e] = fma(h.g2 * gd, gd, (double)fv * uv);
+        md[e] = product_sum((double)fm, um, h.g1, gd);
+        vd[e] = product_sum((double)fv, uv, h.g2 * gd, gd);
         const uint32_t am = (uint32_t)__double2hiint(md[e]) & 0x7fffffffu, av = (uint32_t)__double2hiint(vd[e]);
         hm = am > hm ? am : hm;
         hv = av > hv ? av : hv;
@@ -336,21 +383,10 @@ __device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper8 &h)
     const int xm = 127 - s1m - kM.shift, xv = 127 - s1v - kV.shift;
     const uint32_t place = at.place + i;
     const uint32_t w0m = place * kPlaceM + s.t * kStepM, w0v = place * kPlaceV + s.t * kStepV;
-    Vec<uint32_t, 2> om = 0, ov = 0;
-    // behind the tensor's end gradients and codes are zero, and so are the codes that come out
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const uint32_t off = e < 4 ? e : APART + e - 4;
-        uint32_t a = code_of(md[e], xm, w0m + off * kPlaceM), b = code_of(vd[e], xv, w0v + off * kPlaceV);
-        a = a > kM.most_code ? kM.most_code : a;
-        a |= (uint32_t)__double2hiint(md[e]) >> 24 & 128u;
-        // 1 where v is not zero (written out: as a comparison it takes twice the instructions): a v that vanished under a live m would divide it by eps alone
-        uint32_t live;
-        asm("v_min_u32 %0, 1, %1" : "=v"(live) : "v"(__double2hiint(vd[e])));
-        asm("v_med3_u32 %0, %1, %2, %3" : "=v"(b) : "v"(b), "v"(live), "s"(kV.most_code));
-        om[e / 4] |= a << (8 * (e & 3));
-        ov[e / 4] |= b << (8 * (e & 3));
-    }
+    Vec<uint32_t, 2> om, ov;
+    uint32_t low = 0;
+    encode<false, APART>(md, vd, xm, xv, w0m, w0v, om, ov, low);
+    if (__builtin_expect(low >= 0xfffffff8u, 0)) encode<true, APART>(md, vd, xm, xv, w0m, w0v, om, ov, low);
     if (s1m == 255) om = 0;
     if (s1v == 255) ov = 0;
     if constexpr (APART == 4) {
@@ -466,7 +502,8 @@ __global__ __launch_bounds__(kThreads, BITS == 32 ? 6 : 5) void k_adamw_group(co
         }
 }
 
-// moments as float32: what the codes stand for
+// Moments as float32: what the codes stand for.  One workgroup for 1024 elements, in order: 240M elements 384 us (10 bytes each, 6.25
+// TB/s); 8192 workgroups in a loop 486 us.
 __global__ __launch_bounds__(kThreads) void k_moments(const uint8_t *m, const uint8_t *v, const uint8_t *sm, const uint8_t *sv, float *mo,
                                                             float *vo, int64_t n)
 {
@@ -489,7 +526,9 @@ __global__ __launch_bounds__(kThreads) void k_moments(const uint8_t *m, const ui
 
 // ---- the global norm -------------------------------------------------------------------------------------------
 // Squares are summed in float64: no gradient that float32 can hold overflows or vanishes there, so no pass looks for a scale first.
-// Workgroup b always takes the same chunks and its sum has its own place, so the norm is the same bits on every run.
+// Workgroup b always takes the same chunks and its sum has its own place, so the norm is the same bits on every run.  The workgroups
+// sweep the tensors together, 8192 elements each at a time with all loads of a chunk under way: 240M float32 elements 143 us (6.7 TB/s);
+// each in a region of its own 176 us, chunks of 4096 152 us, of 2048 199 us.
 struct NormArgs {
     void *x[kNormTensors];
     int32_t first_chunk[kNormTensors + 1];
@@ -586,6 +625,7 @@ __device__ inline void chunk_scale(T *x, int count, float f)
     if (i < count) x[i] = (T)((float)x[i] * f);
 }
 
+// 240M float32 elements, norm and scaling: 472 us (2.88 GB, 6.1 TB/s); where the norm is small enough nothing is scaled: 143 us.
 __global__ __launch_bounds__(kThreads) void k_grad_clip(const NormArgs a, const double *partials, int n_partials, double max_norm, float *norm_out)
 {
     const double norm = sqrt(sum_partials(partials, n_partials));

@@ -326,7 +326,8 @@ class GroupedAdamW(torch.optim.Optimizer):
         self._ordered = [self._params[i] for i in order]
         self._numel = (ctypes.c_int64 * n)(*(p.numel() for p in self._ordered))
         self._dtype = (ctypes.c_int32 * n)(*(DTYPE_CODES[p.dtype] for p in self._ordered))
-        self._p, self._g, self._count = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)(), (ctypes.c_int64 * n)()
+        self._p = (ctypes.c_uint64 * n)(*(p.data_ptr() for p in self._ordered))      # as they were checked
+        self._g, self._count = (ctypes.c_uint64 * n)(), (ctypes.c_int64 * n)()
         self._gather_args = tuple(ctypes.addressof(x) for x in (self._numel, self._dtype, self._p, self._g, self._count))
         self._launches, first = [], 0
         for grp, dt, rows in plan:

@@ -37,7 +37,8 @@ def round_block(x, first, t, form):
     i = np.arange(first, first + len(x), dtype=np.uint64)
     word = (i * np.uint64(form["place"]) + np.uint64(t * form["step"] % 2 ** 32)) % np.uint64(2 ** 32)
     u = ((word >> np.uint64(15)) | np.uint64(1)).astype(np.float64) / 2 ** 17
-    c = c + ((y - tab[c]) / (tab[c + 1] - tab[c]) + u >= 1.0)
+    place = c + (y - tab[c]) / (tab[c + 1] - tab[c])                           # on the codes' own scale, a float64: rounded once
+    c = np.floor(place + u).astype(np.int64)
     if form is V:
         c = np.where(a > 0, np.maximum(c, 1), c)
     return np.where(x < 0, -1.0, 1.0) * tab[c] * 2.0 ** (scale - 127), scale

@@ -241,6 +241,39 @@ def test_eight_bits_over_the_range_of_float32(scale):
         assert v[0] > 0 and v[5] == 0 and m[5] == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_eight_bit_codes_on_their_borders(dtype):
+    """Gradients chosen so that 0.9 m + 0.1 g lies on the border between two codes as the element's remainder is drawn, up to the last bits of
+    float64: the formula, rounded operation by operation, says which way each goes, and every code has to follow it."""
+    n, t, s0 = 1 << 16, 7, 110
+    rng = np.random.default_rng(5)
+    tab, unit = F.table(F.M), 2.0 ** (s0 - 127)
+    i = np.arange(n, dtype=np.uint64)
+    u = (((i * np.uint64(F.M["place"]) + np.uint64(t * F.M["step"] % 2 ** 32)) % np.uint64(2 ** 32)) >> np.uint64(15) | np.uint64(1)).astype(np.float64) / 2 ** 17
+    old = rng.integers(8, 112, n) + 128 * rng.integers(0, 2, n)                # codes; the first of each block is the largest and sets the scale
+    c = rng.integers(8, 104, n)
+    target = (tab[c] + (1.0 - u) * (tab[c + 1] - tab[c])) * unit * rng.choice([-1.0, 1.0], n)
+    old[::128], target[::128] = 120, 1.5 * 2.0 ** 8 * unit
+    scales = np.full(n // 128, s0, dtype=np.uint8)
+    m0 = F.values(old, scales, F.M)
+    g = torch.tensor(10.0 * target - 9.0 * m0).to(dtype).to(cuda())
+    p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=cuda()))
+    p.grad = g
+    opt = GroupedAdamW([p], state_bits=8, lr=0.0, weight_decay=0.0)
+    sd = opt.state_dict()
+    sd["fused"]["exp_avg"].copy_(torch.tensor(old.astype(np.uint8)))
+    sd["fused"]["exp_avg_scale"].fill_(s0)
+    sd["fused"]["device_state"].copy_(torch.tensor([[t - 1.0, 0.9 ** (t - 1), 0.999 ** (t - 1)]], dtype=torch.float64))
+    opt.load_state_dict(sd)
+    opt.step()
+    _, m1, v1 = F.step(np.zeros(n), f64(g), m0, np.zeros(n), t)
+    if dtype == torch.float32:
+        near = np.abs(np.abs(m1) / np.abs(target) - 1.0) < 2.0 ** -49
+        assert near.mean() > 0.2 and (np.abs(m1) < np.abs(target))[near].any() and (np.abs(m1) >= np.abs(target))[near].any()
+    ms, vs = opt.moments()
+    assert np.array_equal(f64(ms), F.round_flat(m1, 0, t, F.M)[0]) and np.array_equal(f64(vs), F.round_flat(v1, 0, t, F.V)[0])
+
+
 def test_small_changes_are_not_lost_in_eight_bits():
     """b2 = 0.999: g^2 is 30 times v, so v grows by 3 % a step, less than half a code (6 %); rounding to nearest would stop it.  After n
     steps v is 1 + 29 (1 - 0.999^n) times what it was; a code is 12.5 % wide and the error of a step is below one code, kept from adding up by the
