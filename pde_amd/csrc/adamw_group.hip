@@ -18,8 +18,8 @@
 // The arithmetic is float64, whose products, sums and conversions issue as fast as integer operations here (4.4 to 5.4 cycles a
 // wave; float32 additions 2.8): the top 20 bits of a double's mantissa hold the 3 bits of the code and 17 bits of remainder, so
 // rounding is one integer addition on the double's upper word, and it is exact - the codes do not depend on how a compiler
-// contracts a float32 expression.  240M weights: float32 652 us (16 bytes each, 5.9 TB/s), bfloat16 430 us (10 bytes, 5.6 TB/s: its 48
-// vector instructions an element, 335 us of issue, no longer hide under 387 us of memory).
+// contracts a float32 expression.  240M weights: float32 660 us (16 bytes each, 5.8 TB/s), bfloat16 440 us (10 bytes, 5.5 TB/s: its 52
+// vector instructions an element, 360 us of issue, no longer hide under 387 us of memory).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdlib.h>
@@ -251,23 +251,24 @@ __device__ inline int scale_of(uint32_t hi, const Format &f)
     return s < 0 ? 0 : s > f.most_scale ? f.most_scale : s;
 }
 
-// x's magnitude as a code before it is held to the largest: 3 mantissa bits and what the remainder adds to them.  The place y on the
-// codes' scale (8 times the exponent field plus 8 times the fraction) is a float64 too: where its 53 bits end above x's last ones they are rounded,
-// and a y that is so rounded up to the next 2^-17 carries into the sum.  NEAR does that; without it `low` collects x's lower word, which
-// says whether any x is near enough (8 or fewer units below) for it to matter.
-template <bool NEAR>
-__device__ inline uint32_t code_of(double x, int exponent, uint32_t w, uint32_t &low)
+// x's magnitude as a code before it is held to the largest: 3 mantissa bits and what the remainder adds to them.  `near` collects how far
+// the sum's lower 17 bits came.
+__device__ inline uint32_t code_of(double x, int exponent, uint32_t w, uint32_t &near)
 {
-    const double scaled = ldexp(fabs(x), exponent);
-    uint32_t hi = (uint32_t)__double2hiint(scaled);
-    const uint32_t lo = (uint32_t)__double2loint(scaled);
-    if constexpr (NEAR) {
-        const uint32_t e = hi >> 20, half = e >= 16 ? 8u : e >= 8 ? 4u : e >= 4 ? 2u : e >= 2 ? 1u : 0u;   // half a unit of y's last place, in units of x's
-        if (half && lo >= 0u - half) ++hi;
-    } else {
-        low = lo > low ? lo : low;
-    }
-    return (hi + (w >> 15 | 1u)) >> 17;
+    const uint32_t t = (uint32_t)__double2hiint(ldexp(fabs(x), exponent)) + (w >> 15 | 1u);
+    near = t << 15 > near ? t << 15 : near;
+    return t >> 17;
+}
+
+// The place y on the codes' scale (8 times the exponent field plus 8 times the fraction) is a float64 too, and the larger it is the fewer
+// of x's last bits it has.  An x so near below a multiple of 2^-17 codes that y is rounded up to it takes that value.  It only
+// matters where the sum lacks one to the next code (all 17 bits are set): about one wave in 130 looks.
+__device__ inline double settled(double x, int exponent)
+{
+    const uint32_t hi = (uint32_t)__double2hiint(x), lo = (uint32_t)__double2loint(x);
+    const int field = (int)((hi & 0x7fffffffu) >> 20) + exponent;
+    const uint32_t half = field >= 16 ? 8u : field >= 8 ? 4u : field >= 4 ? 2u : field >= 2 ? 1u : 0u;   // half a unit of y's last place, in x's
+    return half && lo >= 0u - half ? __hiloint2double((int)(hi + 1), 0) : x;
 }
 
 // the sequences that round: golden ratio, sqrt(2) over the elements; the two-dimensional analogue of the golden ratio over the steps
@@ -305,28 +306,6 @@ __device__ inline void store_runs(T *p, Vec<T, 8> x, int have)
     if constexpr (APART == 4) return store_some<FULL, 8>(p, x, have);
     store_some<FULL, 4>(p, __builtin_shufflevector(x, x, 0, 1, 2, 3), have);
     store_some<FULL, 4>(p + APART, __builtin_shufflevector(x, x, 4, 5, 6, 7), have - APART);
-}
-
-// behind the tensor's end gradients and codes are zero, and so are the codes that come out
-template <bool NEAR, int APART>
-__device__ inline void encode(const double (&md)[8], const double (&vd)[8], int xm, int xv, uint32_t w0m, uint32_t w0v, Vec<uint32_t, 2> &om,
-                              Vec<uint32_t, 2> &ov, uint32_t &low)
-{
-    om = 0;
-    ov = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t off = e < 4 ? e : APART + e - 4;
-        uint32_t a = code_of<NEAR>(md[e], xm, w0m + off * kPlaceM, low), b = code_of<NEAR>(vd[e], xv, w0v + off * kPlaceV, low);
-        a = a > kM.most_code ? kM.most_code : a;
-        a |= (uint32_t)__double2hiint(md[e]) >> 24 & 128u;
-        // 1 where v is not zero (written out: as a comparison it takes twice the instructions): a v that vanished under a live m would divide it by eps alone
-        uint32_t live;
-        asm("v_min_u32 %0, 1, %1" : "=v"(live) : "v"(__double2hiint(vd[e])));
-        asm("v_med3_u32 %0, %1, %2, %3" : "=v"(b) : "v"(b), "v"(live), "s"(kV.most_code));
-        om[e / 4] |= a << (8 * (e & 3));
-        ov[e / 4] |= b << (8 * (e & 3));
-    }
 }
 
 template <bool FULL, bool MASTER, class T>
@@ -382,11 +361,36 @@ __device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper8 &h)
     const int s1m = scale_of(row_max(hm), kM), s1v = scale_of(row_max(hv), kV);
     const int xm = 127 - s1m - kM.shift, xv = 127 - s1v - kV.shift;
     const uint32_t place = at.place + i;
-    const uint32_t w0m = place * kPlaceM + s.t * kStepM, w0v = place * kPlaceV + s.t * kStepV;
+    uint32_t w0m = place * kPlaceM + s.t * kStepM, w0v = place * kPlaceV + s.t * kStepV;
     Vec<uint32_t, 2> om, ov;
-    uint32_t low = 0;
-    encode<false, APART>(md, vd, xm, xv, w0m, w0v, om, ov, low);
-    if (__builtin_expect(low >= 0xfffffff8u, 0)) encode<true, APART>(md, vd, xm, xv, w0m, w0v, om, ov, low);
+    // behind the tensor's end gradients and codes are zero, and so are the codes that come out
+#pragma unroll 1
+    for (bool again = false;;) {
+        asm("" : "+v"(w0m), "+v"(w0v));         // or all 16 of the sums below are made before the loop, which would take registers that are not there
+        uint32_t near = 0;
+        om = 0;
+        ov = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t off = e < 4 ? e : APART + e - 4;
+            uint32_t a = code_of(md[e], xm, w0m + off * kPlaceM, near), b = code_of(vd[e], xv, w0v + off * kPlaceV, near);
+            a = a > kM.most_code ? kM.most_code : a;
+            a |= (uint32_t)__double2hiint(md[e]) >> 24 & 128u;
+            // 1 where v is not zero (written out: as a comparison it takes twice the instructions): a v that vanished under a live m would divide it by eps alone
+            uint32_t live;
+            asm("v_min_u32 %0, 1, %1" : "=v"(live) : "v"(__double2hiint(vd[e])));
+            asm("v_med3_u32 %0, %1, %2, %3" : "=v"(b) : "v"(b), "v"(live), "s"(kV.most_code));
+            om[e / 4] |= a << (8 * (e & 3));
+            ov[e / 4] |= b << (8 * (e & 3));
+        }
+        if (__builtin_expect(again || near < 0xffff8000u, 1)) break;
+        again = true;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            md[e] = settled(md[e], xm);
+            vd[e] = settled(vd[e], xv);
+        }
+    }
     if (s1m == 255) om = 0;
     if (s1v == 255) ov = 0;
     if constexpr (APART == 4) {
