@@ -122,13 +122,14 @@ PyObject *gather(PyObject *, PyObject *args)
 }
 
 // describe(tensors, of_grads, x, numel, dtype) -> (how many, [(place in the arrays, index) of those that are neither contiguous nor another
-// order of the same memory], index of their GPU, elements in all); of_grads: the gradients of those tensors that have one
+// order of the same memory], index of their GPU, elements in all); of_grads: the gradients of those tensors that have one, 2: and they
+// count as written to
 PyObject *describe(PyObject *, PyObject *args)
 {
     PyObject *list;
     int of_grads;
     unsigned long long a_x, a_numel, a_dtype;
-    if (!PyArg_ParseTuple(args, "O!pKKK", &PyList_Type, &list, &of_grads, &a_x, &a_numel, &a_dtype)) return nullptr;
+    if (!PyArg_ParseTuple(args, "O!iKKK", &PyList_Type, &list, &of_grads, &a_x, &a_numel, &a_dtype)) return nullptr;
     return guarded([&]() -> PyObject * {
         uint64_t *x = (uint64_t *)(uintptr_t)a_x;
         int64_t *numel = (int64_t *)(uintptr_t)a_numel;
@@ -175,31 +176,18 @@ PyObject *describe(PyObject *, PyObject *args)
             }
             ++k;
         }
+        if (of_grads == 2)
+            for (Py_ssize_t i = 0; i < n; ++i) {
+                const at::Tensor &g = THPVariable_Unpack(PyList_GET_ITEM(list, i)).grad();
+                if (g.defined() && !g.is_inference()) g.unsafeGetTensorImpl()->bump_version();
+            }
         if (k == 0) return Py_BuildValue("(nNOi)", k, other, Py_None, 0);
         return Py_BuildValue("(nNnL)", k, other, (Py_ssize_t)device.index(), (long long)total);
     });
 }
 
-// grads_written(params): the gradients of those that have one were written to in place
-PyObject *grads_written(PyObject *, PyObject *list)
-{
-    if (!PyList_Check(list)) {
-        PyErr_SetString(PyExc_TypeError, "a list is needed");
-        return nullptr;
-    }
-    return guarded([&]() -> PyObject * {
-        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-            if (!tensor_at(list, i, "parameter")) return nullptr;
-            const at::Tensor &g = THPVariable_Unpack(PyList_GET_ITEM(list, i)).grad();
-            if (g.defined() && !g.is_inference()) g.unsafeGetTensorImpl()->bump_version();
-        }
-        Py_RETURN_NONE;
-    });
-}
-
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, nullptr},
                          {"describe", describe, METH_VARARGS, nullptr},
-                         {"grads_written", grads_written, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

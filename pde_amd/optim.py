@@ -145,10 +145,10 @@ def _flat(t):
 
 
 class _TensorList:
-    """Tensors, or with `of_grads` the gradients of those that have one, as the C interface takes them: host arrays of addresses, lengths
+    """Tensors, or with `of_grads` the gradients of those that have one (2: to be written to), as the C interface takes them: host arrays of addresses, lengths
     and types.  `back`: (tensor, copy) of those whose memory has gaps or overlaps, the copy is what the arrays name."""
 
-    def __init__(self, tensors, of_grads=False):
+    def __init__(self, tensors, of_grads=0):
         n = len(tensors)
         self.x, self.numel, self.dtype = (ctypes.c_uint64 * n)(), (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
         at = ctypes.addressof(self.x), ctypes.addressof(self.numel), ctypes.addressof(self.dtype)
@@ -200,7 +200,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     if not max_norm >= 0.0:
         raise ValueError("max_norm is %r: 0 or more is needed" % max_norm)
     parameters = _as_list(parameters)
-    lst = _TensorList(parameters, of_grads=True)
+    lst = _TensorList(parameters, of_grads=2)
     if lst.n == 0:
         return torch.tensor(0.0)
     if any(0 in (st for sz, st in zip(g.shape, g.stride()) if sz > 1) for g, _ in lst.back):
@@ -219,7 +219,6 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
         _check(rc, "pinn_grad_clip")
         for g, c in lst.back:
             g.copy_(c)
-    load_tensorlist().grads_written(parameters)
     return norm
 
 

@@ -13,6 +13,7 @@ from pde_amd.optim import GroupedAdamW, clip_grad_norm_, grad_norm
 from conftest import GOLDEN, ROOT
 
 needs_lib = pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="libpinnjet.so not built")
+needs_list = pytest.mark.skipif(not os.path.exists(os.path.join(ROOT, "pde_amd", "_tensorlist.so")), reason="_tensorlist.so not built")
 
 
 def test_formulas_follow_torch():
@@ -52,6 +53,7 @@ def test_eight_bit_format(form):
         assert (F.round_block(tiny, 0, 1, form)[0] > 0).all()
 
 
+@needs_list
 def test_refusals_without_a_gpu():
     p = torch.nn.Parameter(torch.ones(3))
     with pytest.raises(NativeError, match="no CPU fallback"):
@@ -155,6 +157,7 @@ def test_options_that_need_the_grouped_step():
         m.train(1, LBFGS_max_iter=0)
 
 
+@needs_list
 def test_lists_of_tensors():
     """csrc/tensorlist.cpp on CPU tensors: what it reads, which gradients it hands back, what it refuses"""
     import ctypes as C
@@ -177,9 +180,6 @@ def test_lists_of_tensors():
     ps[4].grad = torch.ones(9, 1).t()                                          # another stride of a dimension of one element: the same order
     assert gather() == (4, [2], False) and g[2] == 0 and g[4] == ps[4].grad.data_ptr()
     assert [q._version - b for q, b in zip(ps, before)] == [2, 0, 2, 2, 2, 0]
-    before = [q.grad._version for q in ps[:5]]
-    native.grads_written(ps)
-    assert [q.grad._version - b for q, b in zip(ps, before)] == [1] * 5
     dtype[3] = 1
     with pytest.raises(ValueError, match="parameter 3 is not what it was"):
         gather()
@@ -210,12 +210,14 @@ def test_lists_of_tensors():
     qs = [torch.nn.Parameter(t) for t in (a, a[0], a[1])]
     assert describe(qs, True) == (0, [], None, 0)
     qs[1].grad, qs[2].grad = torch.empty(6, device="meta"), torch.empty(12, device="meta")[::2]
-    assert describe(qs, True) == (2, [(1, 2)], -1, 12)
+    before = [q.grad._version for q in qs[1:]]
+    assert describe(qs, 1) == (2, [(1, 2)], -1, 12) and [q.grad._version for q in qs[1:]] == before
+    assert describe(qs, 2) == (2, [(1, 2)], -1, 12) and [q.grad._version for q in qs[1:]] == [b + 1 for b in before]
     for bad in (a.double(), a.long(), torch.empty(4, 6, layout=torch.sparse_coo, device="meta")):
         with pytest.raises(ValueError, match="tensor 1"):
             describe([a, bad])
     with pytest.raises(ValueError, match="one device"):
         describe([a, torch.empty(2)])
-    for call in (lambda: describe([a, 3]), lambda: native.gather([None] * 6, 0, 0, 0, 0, 0), lambda: describe((a,)), lambda: native.grads_written([a, None]), lambda: native.grads_written((a,))):
+    for call in (lambda: describe([a, 3]), lambda: native.gather([None] * 6, 0, 0, 0, 0, 0), lambda: describe((a,)), lambda: describe([a, None], 2)):
         with pytest.raises(TypeError):
             call()

@@ -357,6 +357,46 @@ def test_two_captured_clippings_on_two_streams():
             assert abs(float(grad_norm([p.grad for p in params])) - 1.0) < 1e-5
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_two_optimizers_at_once(bits):
+    """each on a stream of its own, clipped: nothing is shared between them"""
+    def model(k):
+        params = params_of(make(SIZES + [(300000,)], torch.float32, 130 + k))
+        for p, g in zip(params, make(SIZES + [(300000,)], torch.float32, 140 + k)):
+            p.grad = g
+        return params, GroupedAdamW(params, state_bits=bits, max_norm=0.5 + k, **HYPER)
+    alone, together = [model(k) for k in range(2)], [model(k) for k in range(2)]
+    for _, opt in alone:
+        for _ in range(5):
+            opt.step()
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (_, opt), st in zip(together, streams):
+            with torch.cuda.stream(st):
+                opt.step()
+    torch.cuda.synchronize()
+    for (pa, a), (pb, b) in zip(alone, together):
+        sa, sb = a.state_dict()["fused"], b.state_dict()["fused"]
+        assert all(torch.equal(sa[n], sb[n]) for n in sa) and all(torch.equal(x, y) for x, y in zip(pa, pb))
+        assert torch.equal(a.grad_norm, b.grad_norm) and not a._ticket.any() and not b._ticket.any()
+
+
+def test_scalars_and_empty_parameters_and_none_without_gradients():
+    params = params_of([torch.tensor(0.5, device=cuda()), torch.empty(0, 3, device=cuda()), torch.ones(2, device=cuda())])
+    opt = GroupedAdamW(params, max_norm=1.0, **HYPER)
+    before = opt.state_dict()["fused"]
+    opt.step()                                                                 # nobody has a gradient: nothing happens
+    after = opt.state_dict()["fused"]
+    assert all(torch.equal(before[n], after[n]) for n in before)
+    run(opt, 2, 700)
+    only_empty = GroupedAdamW([params[1]])
+    params[1].grad = torch.empty(0, 3, device=cuda())
+    only_empty.step()
+    assert only_empty.moments()[0].numel() == 0 and GroupedAdamW([params[1]], state_bits=8).moments()[0].numel() == 0
+
+
 def test_step_on_another_stream_and_closure():
     params = params_of(make(SIZES, torch.float32, 60))
     opt = GroupedAdamW(params, max_norm=1.0, **HYPER)
@@ -610,6 +650,8 @@ def test_refusals():
     base = torch.zeros(300, device=cuda())
     with pytest.raises(ValueError, match="share memory"):
         GroupedAdamW([torch.nn.Parameter(base[:200]), torch.nn.Parameter(base[199:])])
+    with pytest.raises(ValueError, match="share memory"), pytest.warns(UserWarning, match="duplicate"):
+        GroupedAdamW([p[0], p[0]])
     with pytest.raises(ValueError, match="gaps"):
         GroupedAdamW([torch.nn.Parameter(base[::2])])
     with pytest.raises(ValueError, match="float64"):
