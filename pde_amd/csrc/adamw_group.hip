@@ -774,7 +774,7 @@ bool small_list(NormArgs &a, void *const *x, const int64_t *numel, const int32_t
         if (total > kSmallElements) return false;
     }
     NormPlan plan;
-    return n <= kSmallTensors && (plan.advance(a, x, numel, dtype, n), true);
+    return (n <= kSmallTensors || total == 0) && (plan.advance(a, x, numel, dtype, n), true);
 }
 
 int launch_sumsq(const void *const *grads, const int64_t *numel, const int32_t *dtype, int n_tensors, double *partials, int64_t n_reserved,
