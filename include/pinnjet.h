@@ -276,9 +276,9 @@ int pinn_adam_step(float *theta, const float *grad, float *exp_avg, float *exp_a
 #define PINN_ADAMW_CHUNK8 2048       /* the same with 8-bit moments */
 #define PINN_ADAMW_MAX_TENSORS 240   /* tensors per call: their addresses are launch arguments */
 #define PINN_ADAMW_TICKET_WORDS 2080 /* words of the ticket buffer */
-#define PINN_NORM_TENSORS 256       /* tensors per launch of the norm */
+#define PINN_NORM_TENSORS 250       /* tensors per launch of the norm */
 #define PINN_NORM_SMALL_TENSORS 64   /* up to so many tensors of so many elements in all, pinn_grad_norm and _clip are */
-#define PINN_NORM_SMALL_ELEMENTS 16384 /* one launch and need no room for partial sums (it may be NULL) */
+#define PINN_NORM_SMALL_ELEMENTS 32768 /* one launch and need no room for partial sums (it may be NULL) */
 #define PINN_NORM_PARTIALS 1024      /* most partial sums per launch of pinn_grad_sumsq */
 
 typedef struct {                     /* PINN_ADAMW_CHUNK32 or _CHUNK8 elements of one tensor, or the rest of it */

@@ -533,12 +533,15 @@ __global__ __launch_bounds__(kThreads) void k_moments(const uint8_t *m, const ui
 // Workgroup b always takes the same chunks and its sum has its own place, so the norm is the same bits on every run.  The workgroups
 // sweep the tensors together, 8192 elements each at a time with all loads of a chunk under way: 240M float32 elements 143 us (6.7 TB/s);
 // each in a region of its own 176 us, chunks of 4096 152 us, of 2048 199 us.
+// Whole words only: from an index into bytes the compiler may make a scalar load whose base and offset are each unaligned (base + k, offset
+// 7 k for word pair k), and scalar loads drop the lowest two bits of each by itself.
 struct NormArgs {
     void *x[kNormTensors];
     int32_t first_chunk[kNormTensors + 1];
-    uint16_t tail[kNormTensors];                // elements of a tensor's last chunk, 1 .. kNormChunk
-    uint8_t dtype[kNormTensors];
+    uint32_t kind[kNormTensors];                // elements of a tensor's last chunk, 1 .. kNormChunk, and its type above 16 bits
     int32_t n_tensors, first_partial;
+    __host__ __device__ int tail(int k) const { return (int)(kind[k] & 0xffffu); }
+    __host__ __device__ int dtype(int k) const { return (int)(kind[k] >> 16); }
 };
 static_assert(sizeof(NormArgs) + 48 <= 4096, "a launch's arguments");
 
@@ -586,9 +589,9 @@ __global__ __launch_bounds__(kThreads) void k_grad_sumsq(const NormArgs a, doubl
     for (int64_t ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
         const int k = find_tensor(a, ch);
         const int64_t base = (ch - a.first_chunk[k]) * kNormChunk;
-        const int count = ch + 1 == a.first_chunk[k + 1] ? a.tail[k] : kNormChunk;
-        if (a.dtype[k] == PINN_F32) s += chunk_sumsq((const float *)a.x[k] + base, count);
-        else if (a.dtype[k] == PINN_BF16) s += chunk_sumsq((const __bf16 *)a.x[k] + base, count);
+        const int count = ch + 1 == a.first_chunk[k + 1] ? a.tail(k) : kNormChunk;
+        if (a.dtype(k) == PINN_F32) s += chunk_sumsq((const float *)a.x[k] + base, count);
+        else if (a.dtype(k) == PINN_BF16) s += chunk_sumsq((const __bf16 *)a.x[k] + base, count);
         else s += chunk_sumsq((const _Float16 *)a.x[k] + base, count);
     }
     __shared__ double part[kThreads / 64];
@@ -640,41 +643,59 @@ __global__ __launch_bounds__(kThreads) void k_grad_clip(const NormArgs a, const 
     for (int64_t ch = blockIdx.x; ch < n_chunks; ch += gridDim.x) {
         const int k = find_tensor(a, ch);
         const int64_t base = (ch - a.first_chunk[k]) * kNormChunk;
-        const int count = ch + 1 == a.first_chunk[k + 1] ? a.tail[k] : kNormChunk;
-        if (a.dtype[k] == PINN_F32) chunk_scale((float *)a.x[k] + base, count, f);
-        else if (a.dtype[k] == PINN_BF16) chunk_scale((__bf16 *)a.x[k] + base, count, f);
+        const int count = ch + 1 == a.first_chunk[k + 1] ? a.tail(k) : kNormChunk;
+        if (a.dtype(k) == PINN_F32) chunk_scale((float *)a.x[k] + base, count, f);
+        else if (a.dtype(k) == PINN_BF16) chunk_scale((__bf16 *)a.x[k] + base, count, f);
         else chunk_scale((_Float16 *)a.x[k] + base, count, f);
     }
 }
 
-// Few elements: ONE workgroup forms the norm and, with max_norm >= 0, scales, a wave to a tensor at a time.  A launch is 3.7 us at the
-// host, so for a small net the second one is a third of the call.
-constexpr int kSmallThreads = 1024, kSmallTensors = PINN_NORM_SMALL_TENSORS;
+// Few elements: ONE workgroup forms the norm and, with max_norm >= 0, scales.  A launch is 3.7 us at the host, so for a small net the second one
+// is a quarter of the call (10 tensors: clipping 10.4 us, in two launches 13.2).  The tensors are cut into runs of 256 elements, which the 16
+// waves take in turn: up to 32768 elements the kernel hides behind the host's next call, with 65536 a call takes 17.6 us, with 131072 31.7.
+constexpr int kSmallThreads = 1024, kSmallTensors = PINN_NORM_SMALL_TENSORS, kRun = 256;
 constexpr int64_t kSmallElements = PINN_NORM_SMALL_ELEMENTS;
+static_assert(kSmallTensors == 64, "a lane for each tensor");
 
-template <class T, class F>
-__device__ inline void wave_over(T *x, int n, F f)
+__device__ inline int length_of(const NormArgs &a, int k)
 {
-#pragma unroll 4
-    for (int i = threadIdx.x & 63; i < n; i += 64) f(x[i]);
+    return (a.first_chunk[k + 1] - a.first_chunk[k] - 1) * kNormChunk + a.tail(k);
 }
 
+// f(elements of a lane, how many there are, their address) for all runs; first[k]: runs before tensor k
 template <class F>
-__device__ inline void waves_over(const NormArgs &a, F f)
+__device__ inline void over_runs(const NormArgs &a, const int *first, F f)
 {
-    for (int k = threadIdx.x >> 6; k < a.n_tensors; k += kSmallThreads / 64) {
-        const int n = (a.first_chunk[k + 1] - a.first_chunk[k] - 1) * kNormChunk + a.tail[k];
-        if (a.dtype[k] == PINN_F32) wave_over((float *)a.x[k], n, f);
-        else if (a.dtype[k] == PINN_BF16) wave_over((__bf16 *)a.x[k], n, f);
-        else wave_over((_Float16 *)a.x[k], n, f);
+    const int lane = threadIdx.x & 63, upto = first[lane + 1], total = first[kSmallTensors];
+    for (int j = threadIdx.x >> 6; j < total; j += kSmallThreads / 64) {
+        const int k = __popcll(__ballot(upto <= j));           // the tensors that end before run j
+        const int i = (j - first[k]) * kRun + lane * 4, have = length_of(a, k) - i;
+        if (a.dtype(k) == PINN_F32) f(load_some<false, 4>((float *)a.x[k] + i, have), have, (float *)a.x[k] + i);
+        else if (a.dtype(k) == PINN_BF16) f(load_some<false, 4>((__bf16 *)a.x[k] + i, have), have, (__bf16 *)a.x[k] + i);
+        else f(load_some<false, 4>((_Float16 *)a.x[k] + i, have), have, (_Float16 *)a.x[k] + i);
     }
 }
 
 __global__ __launch_bounds__(kSmallThreads) void k_norm_small(const NormArgs a, double max_norm, float *norm_out)
 {
+    __shared__ int first[kSmallTensors + 1];
     __shared__ double part[kSmallThreads / 64];
+    if (threadIdx.x < kSmallTensors) {
+        const int k = threadIdx.x;
+        int runs = k < a.n_tensors ? (length_of(a, k) + kRun - 1) / kRun : 0;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int before = __shfl_up(runs, d);
+            if (k >= d) runs += before;
+        }
+        first[k + 1] = runs;
+        if (k == 0) first[0] = 0;
+    }
+    __syncthreads();
     double s = 0.0;
-    waves_over(a, [&](auto &x) { s = fma((double)(float)x, (double)(float)x, s); });
+    over_runs(a, first, [&](auto x, int, auto *) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = fma((double)(float)x[e], (double)(float)x[e], s);
+    });
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -685,7 +706,12 @@ __global__ __launch_bounds__(kSmallThreads) void k_norm_small(const NormArgs a, 
     if (max_norm < 0.0) return;
     const float f = (float)clip_factor(norm, max_norm);
     if (f == 1.0f) return;
-    waves_over(a, [&](auto &x) { x = (std::remove_reference_t<decltype(x)>)((float)x * f); });
+    over_runs(a, first, [&](auto x, int have, auto *at) {
+        typedef std::remove_reference_t<decltype(*at)> T;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (T)((float)x[e] * f);
+        store_some<false, 4>(at, x, have);
+    });
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
@@ -723,8 +749,7 @@ struct NormPlan {
             if (chunks + more > INT32_MAX) break;
             const int k = a.n_tensors++;
             a.x[k] = x[next];
-            a.tail[k] = (uint16_t)(numel[next] - (more - 1) * kNormChunk);
-            a.dtype[k] = (uint8_t)dtype[next];
+            a.kind[k] = (uint32_t)(numel[next] - (more - 1) * kNormChunk) | (uint32_t)dtype[next] << 16;
             a.first_chunk[k] = (int32_t)chunks;
             chunks += more;
         }

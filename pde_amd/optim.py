@@ -193,7 +193,7 @@ def grad_norm(tensors):
 
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     """Scales the gradients of `parameters` in place so that their global 2-norm is at most `max_norm`, and returns the norm
-    they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 256 tensors (one for few elements),
+    they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 250 tensors (one for few elements),
     without a copy of the gradients.  The factor is min(1, max_norm / (norm + 1e-6)); with a norm that is not finite it is 0 or NaN, as
     there; `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError)."""
     max_norm = float(max_norm)

@@ -114,7 +114,7 @@ def test_c_entries_refuse_without_a_gpu():
     assert lib.pinn_adamw_moments(None, None, None, None, None, None, 0, None) == 0
 
     assert lib.pinn_grad_norm_partials(-1) == INVALID and lib.pinn_grad_norm_partials(0) == 0
-    assert lib.pinn_grad_norm_partials(256) == 1024 and lib.pinn_grad_norm_partials(257) == 2048
+    assert lib.pinn_grad_norm_partials(250) == 1024 and lib.pinn_grad_norm_partials(251) == 2048
     count = ctypes.c_int32()
     n2, f32 = (ctypes.c_int64 * 2)(100, 100), (ctypes.c_int32 * 2)(0, 0)
 

@@ -597,10 +597,10 @@ def test_clip_grad_norm(max_norm):
             assert np.array_equal(f64(p.grad), g)
 
 
-@pytest.mark.parametrize("n_tensors,size", [(1, 1), (10, 785), (64, 256), (65, 252), (16, 1024), (17, 1024), (1, 16384), (1, 16385), (700, 3)])
+@pytest.mark.parametrize("n_tensors,size", [(1, 1), (10, 785), (64, 256), (65, 252), (16, 1024), (1, 16385), (32, 1024), (33, 1024), (1, 32768), (1, 32769), (700, 3)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_clip_grad_norm_around_the_one_launch_form(dtype, n_tensors, size):
-    """few elements take one workgroup, 16384 elements and 64 tensors are its limits"""
+    """few elements take one workgroup, 32768 elements and 64 tensors are its limits"""
     params = params_of(make([(size,)] * n_tensors, dtype, 106))
     for p, g in zip(params, make([(size,)] * n_tensors, dtype, 107, 2.0)):
         p.grad = g
@@ -613,7 +613,7 @@ def test_clip_grad_norm_around_the_one_launch_form(dtype, n_tensors, size):
         assert (np.abs(f64(p.grad) - g * f) <= 2 * H * np.abs(g * f) + half_step(p.dtype, g * f)).all()
 
 
-@pytest.mark.parametrize("size", [1000, 20000])
+@pytest.mark.parametrize("size", [1000, 50000])
 def test_clip_grad_norm_of_norms_that_are_not_finite(size):
     for bad in (float("nan"), float("inf")):
         p = params_of(make([(size,)], torch.float32, 110))[0]
