@@ -613,6 +613,21 @@ def test_clip_grad_norm_around_the_one_launch_form(dtype, n_tensors, size):
         assert (np.abs(f64(p.grad) - g * f) <= 2 * H * np.abs(g * f) + half_step(p.dtype, g * f)).all()
 
 
+@pytest.mark.parametrize("dtype,n_tensors,size", [(torch.bfloat16, 600, 24579), (torch.float32, 3, 5_000_003), (torch.float16, 513, 32768)])
+def test_clip_grad_norm_of_many_chunks(dtype, n_tensors, size):
+    """workgroups that take several chunks, and launches whose partial sums (2400 and 2052) are added up once"""
+    flat = make([(n_tensors * size,)], dtype, 108)[0]
+    params = [torch.nn.Parameter(t) for t in torch.empty_like(flat).view(n_tensors, size).unbind()]
+    for p, g in zip(params, flat.view(n_tensors, size).unbind()):
+        p.grad = g
+    had = f64(flat)
+    norm, f = F.clip_factor([had], 0.5)
+    assert torch.equal(grad_norm([p.grad for p in params]), clip_grad_norm_(params, 1e9)) and np.array_equal(f64(flat), had)
+    assert abs(float(clip_grad_norm_(params, 0.5)) - norm) <= 2 * H * norm
+    want = had * f
+    assert (np.abs(f64(flat) - want) <= 2 * H * np.abs(want) + half_step(dtype, want)).all()
+
+
 @pytest.mark.parametrize("size", [1000, 50000])
 def test_clip_grad_norm_of_norms_that_are_not_finite(size):
     for bad in (float("nan"), float("inf")):
