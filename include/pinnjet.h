@@ -275,6 +275,7 @@ int pinn_adam_step(float *theta, const float *grad, float *exp_avg, float *exp_a
 #define PINN_ADAMW_CHUNK32 1024      /* elements a workgroup takes at a time, with float32 moments */
 #define PINN_ADAMW_CHUNK8 2048       /* the same with 8-bit moments */
 #define PINN_ADAMW_MAX_TENSORS 240   /* tensors per call: their addresses are launch arguments */
+#define PINN_ADAMW_MAX_CHUNKS 16777215 /* chunks per call: a launch holds fewer than 2^32 threads, 256 for each chunk */
 #define PINN_ADAMW_TICKET_WORDS 2080 /* words of the ticket buffer */
 #define PINN_NORM_TENSORS 250       /* tensors per launch of the norm */
 #define PINN_NORM_SMALL_TENSORS 64   /* up to so many tensors of so many elements in all, pinn_grad_norm and _clip are */

@@ -44,7 +44,7 @@ class PinnAdamWGroup(ctypes.Structure):
 
 # include/pinnjet.h: dtype codes and the constants of the AdamW step over many tensors
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS = 128, 1024, 2048, 240, 2080
+ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_MAX_TENSORS, ADAMW_MAX_CHUNKS, ADAMW_TICKET_WORDS = 128, 1024, 2048, 240, 2 ** 24 - 1, 2080
 NORM_SMALL_TENSORS, NORM_SMALL_ELEMENTS = 64, 32768
 ERR_OVERLAP = -7
 

@@ -507,7 +507,9 @@ __global__ __launch_bounds__(kThreads, BITS == 32 ? 6 : 5) void k_adamw_group(co
 }
 
 // Moments as float32: what the codes stand for.  One workgroup for 1024 elements, in order: 240M elements 384 us (10 bytes each, 6.25
-// TB/s); 8192 workgroups in a loop 486 us.
+// TB/s); 8192 workgroups in a loop 486 us.  A launch holds fewer than 2^32 threads.
+constexpr int64_t kMomentsLaunch = (int64_t)1 << 33;
+static_assert(kMomentsLaunch / 4 < (int64_t)1 << 32 && kMomentsLaunch % kBlock == 0, "threads of a launch; scales begin with it");
 __global__ __launch_bounds__(kThreads) void k_moments(const uint8_t *m, const uint8_t *v, const uint8_t *sm, const uint8_t *sv, float *mo,
                                                             float *vo, int64_t n)
 {
@@ -890,7 +892,7 @@ extern "C" int pinn_adamw_group_step(const PinnAdamWGroup *d, void *const *param
     if (d->n_tensors < 0 || d->n_tensors > kMaxTensors || d->n_chunks < 0 || !valid_dtype(d->dtype) ||
         (d->state_bits != 32 && d->state_bits != 8) || d->n_partials < 0 || (d->master && d->dtype == PINN_F32))
         return PINN_ERR_INVALID_DESC;
-    if (d->n_chunks > INT32_MAX) return PINN_ERR_TOO_LARGE;
+    if (d->n_chunks > PINN_ADAMW_MAX_CHUNKS) return PINN_ERR_TOO_LARGE;
     if (d->n_tensors == 0 || d->n_chunks == 0) return PINN_OK;
     if (!d->chunks || !d->rows || !d->exp_avg || !d->exp_avg_sq || !d->device_state || !d->ticket) return PINN_ERR_NULL;
     if (d->state_bits == 8 && (!d->exp_avg_scale || !d->exp_avg_sq_scale)) return PINN_ERR_NULL;
@@ -944,9 +946,11 @@ extern "C" int pinn_adamw_moments(const uint8_t *exp_avg, const uint8_t *exp_avg
     if (n < 0 || n % kBlock) return PINN_ERR_INVALID_DESC;
     if (n == 0) return PINN_OK;
     if (!exp_avg || !exp_avg_sq || !exp_avg_scale || !exp_avg_sq_scale || !exp_avg_out || !exp_avg_sq_out) return PINN_ERR_NULL;
-    const int64_t groups = (n / 4 + kThreads - 1) / kThreads;
-    if (groups > INT32_MAX) return PINN_ERR_TOO_LARGE;
-    hipLaunchKernelGGL(k_moments, dim3((unsigned)groups), dim3(kThreads), 0, (hipStream_t)stream, exp_avg,
-                       exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, exp_avg_out, exp_avg_sq_out, n);
+    if (n > (int64_t)INT32_MAX * 4 * kThreads) return PINN_ERR_TOO_LARGE;
+    for (int64_t at = 0; at < n; at += kMomentsLaunch) {
+        const int64_t more = std::min(n - at, kMomentsLaunch), groups = (more / 4 + kThreads - 1) / kThreads;
+        hipLaunchKernelGGL(k_moments, dim3((unsigned)groups), dim3(kThreads), 0, (hipStream_t)stream, exp_avg + at, exp_avg_sq + at,
+                           exp_avg_scale + at / kBlock, exp_avg_sq_scale + at / kBlock, exp_avg_out + at, exp_avg_sq_out + at, more);
+    }
     return launch_error();
 }

@@ -17,8 +17,8 @@ import numpy as np
 import torch
 import torch.optim.optimizer as _hooks
 
-from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, DTYPE_CODES,
-                      ERR_OVERLAP, NORM_SMALL_ELEMENTS, NORM_SMALL_TENSORS, NativeError, PinnAdamWGroup, _check, _cur_stream, _on,
+from ._native import (ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_CHUNKS, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS,
+                      DTYPE_CODES, ERR_OVERLAP, NORM_SMALL_ELEMENTS, NORM_SMALL_TENSORS, NativeError, PinnAdamWGroup, _check, _cur_stream, _on,
                       load_library, load_tensorlist)
 
 
@@ -173,6 +173,21 @@ def _partials(n, device):
     return torch.empty(room, dtype=torch.float64, device=device), room
 
 
+def _runs(rows, numel, chunk):
+    """`rows`, tensors of `numel` elements, cut into what one launch of the step takes"""
+    runs, chunks = [], 0
+    for i, n in zip(rows, numel):
+        more = -(-n // chunk)
+        if more > ADAMW_MAX_CHUNKS:
+            raise ValueError("parameter %d has %d elements, a launch takes %d" % (i, n, ADAMW_MAX_CHUNKS * chunk))
+        if not runs or len(runs[-1]) == ADAMW_MAX_TENSORS or chunks + more > ADAMW_MAX_CHUNKS:
+            runs.append([])
+            chunks = 0
+        runs[-1].append(i)
+        chunks += more
+    return runs
+
+
 def _as_list(tensors):
     return [tensors] if torch.is_tensor(tensors) else list(tensors)
 
@@ -223,7 +238,8 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
 
 
 class GroupedAdamW(torch.optim.Optimizer):
-    """AdamW over many tensors at once: one launch per 240 tensors of one group and type.
+    """AdamW over many tensors at once: one launch per 240 tensors (or 2^24 chunks of 1024 elements, 2048 with 8-bit moments) of one
+    group and type.
 
     torch.optim.AdamW's constructor arguments and update rule (decoupled weight decay, no amsgrad; `weight_decay=0` is Adam), plus
 
@@ -255,6 +271,7 @@ class GroupedAdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         for grp in self.param_groups:
             self._hyper(grp)
+        self._chunk = ADAMW_CHUNK32 if state_bits == 32 else ADAMW_CHUNK8
         self._params = [p for grp in self.param_groups for p in grp["params"]]
         self.device = self._params[0].device
         if self.device.type != "cuda":
@@ -319,7 +336,7 @@ class GroupedAdamW(torch.optim.Optimizer):
             first += len(grp["params"])
             for dt in DTYPE_CODES:
                 mine = [i for i in rows if self._params[i].dtype == dt]
-                plan += [(grp, dt, mine[a:a + ADAMW_MAX_TENSORS]) for a in range(0, len(mine), ADAMW_MAX_TENSORS)]
+                plan += [(grp, dt, run) for run in _runs(mine, [self._params[i].numel() for i in mine], self._chunk)]
         order = [i for _, _, rows in plan for i in rows]
         n = len(order)
         self._ordered = [self._params[i] for i in order]
@@ -334,7 +351,7 @@ class GroupedAdamW(torch.optim.Optimizer):
             first += len(rows)
 
     def _launch(self, grp, dtype, rows, first):
-        chunk = ADAMW_CHUNK32 if self.state_bits == 32 else ADAMW_CHUNK8
+        chunk = self._chunk
         numel = np.array([self._params[i].numel() for i in rows], dtype=np.int64)
         count = -(-numel // chunk)
         k = np.repeat(np.arange(len(rows)), count)

@@ -8,8 +8,8 @@ import pytest
 import torch
 
 import adamw_formulas as F
-from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, NORM_SMALL_ELEMENTS, NORM_SMALL_TENSORS, NativeError, PinnAdamWGroup, load_library
-from pde_amd.optim import GroupedAdamW, clip_grad_norm_, grad_norm
+from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_CHUNKS, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, NORM_SMALL_ELEMENTS, NORM_SMALL_TENSORS, NativeError, PinnAdamWGroup, load_library
+from pde_amd.optim import GroupedAdamW, _runs, clip_grad_norm_, grad_norm
 from conftest import GOLDEN, ROOT
 
 needs_lib = pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="libpinnjet.so not built")
@@ -80,7 +80,7 @@ def test_refusals_without_a_gpu():
 def test_c_entries_refuse_without_a_gpu():
     lib = load_library()
     header = open(os.path.join(ROOT, "include", "pinnjet.h")).read()
-    for name, value in (("PINN_ADAMW_BLOCK", ADAMW_BLOCK), ("PINN_ADAMW_CHUNK32", ADAMW_CHUNK32), ("PINN_ADAMW_CHUNK8", ADAMW_CHUNK8), ("PINN_ADAMW_MAX_TENSORS", ADAMW_MAX_TENSORS),
+    for name, value in (("PINN_ADAMW_BLOCK", ADAMW_BLOCK), ("PINN_ADAMW_CHUNK32", ADAMW_CHUNK32), ("PINN_ADAMW_CHUNK8", ADAMW_CHUNK8), ("PINN_ADAMW_MAX_TENSORS", ADAMW_MAX_TENSORS), ("PINN_ADAMW_MAX_CHUNKS", ADAMW_MAX_CHUNKS),
                         ("PINN_ADAMW_TICKET_WORDS", ADAMW_TICKET_WORDS), ("PINN_NORM_SMALL_TENSORS", NORM_SMALL_TENSORS),
                         ("PINN_NORM_SMALL_ELEMENTS", NORM_SMALL_ELEMENTS)):
         assert "#define %s %d " % (name, value) in header
@@ -100,7 +100,7 @@ def test_c_entries_refuse_without_a_gpu():
     for kw in (dict(chunks=None), dict(rows=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(device_state=None), dict(ticket=None),
                dict(state_bits=8), dict(n_partials=4)):
         assert group(**kw) == NULL, kw
-    assert group(n_chunks=1 << 40) == LARGE
+    assert group(n_chunks=1 << 40) == LARGE and group(n_chunks=1 << 24) == LARGE          # 2^24 workgroups of 256: 2^32 threads
     assert lib.pinn_adamw_moments(16, 16, 16, 16, 16, 16, 1 << 50, None) == LARGE
     assert group(n_tensors=0) == 0 and group(n_chunks=0) == 0
     d = PinnAdamWGroup(n_tensors=1, n_chunks=1, state_bits=32, chunks=16, rows=16, exp_avg=16, exp_avg_sq=16, device_state=16, ticket=16)
@@ -137,6 +137,19 @@ def test_c_entries_refuse_without_a_gpu():
     assert clip(x=(ctypes.c_uint64 * 2)(4096, 4096 + 396)) == OVERLAP and clip(x=(ctypes.c_uint64 * 2)(8192, 8192)) == OVERLAP
     assert clip(x=(ctypes.c_uint64 * 2)(4096 + 396, 4096)) == OVERLAP
     assert lib.pinn_error_string(OVERLAP) == b"two tensors share memory"
+
+
+def test_what_a_launch_takes():
+    """240 tensors, and fewer than 2^24 chunks"""
+    assert _runs([], [], 1024) == []
+    assert [len(r) for r in _runs(list(range(500)), [5] * 500, 1024)] == [240, 240, 20]
+    half = (1 << 23) * 1024
+    assert _runs([3, 7, 8, 9], [half, half, 0, 1], 1024) == [[3], [7, 8, 9]]
+    assert _runs([3, 7, 8], [half, half - 1024, 1], 1024) == [[3, 7], [8]]
+    assert _runs([3, 7, 8], [half, half, half], 2048) == [[3, 7, 8]]
+    assert _runs([0], [2 * half - 1024], 1024) == [[0]]
+    with pytest.raises(ValueError, match="elements"):
+        _runs([0], [2 * half - 1023], 1024)
 
 
 def test_options_that_need_the_grouped_step():

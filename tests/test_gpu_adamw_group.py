@@ -11,6 +11,7 @@ import pytest
 import torch
 
 import adamw_formulas as F
+from pde_amd._native import _cur_stream, load_library
 from pde_amd.optim import FusedAdam, GroupedAdamW, clip_grad_norm_, grad_norm
 
 pytestmark = pytest.mark.gpu
@@ -504,6 +505,36 @@ def test_clipping_before_the_step_is_clipping_inside_it(bits):
         assert abs(float(norm) / float(ob.grad_norm) - 1) <= 2 * H
     for p, q in zip(a, b):
         assert ((p - q).abs() <= n_steps * (4 * H * q.abs() + 24 * H * HYPER["lr"] * 10)).all()   # |U| <= 10 lr, generously: |m| / sqrt(v) hat is near 1
+
+
+def test_moments_beyond_one_launch():
+    """2^33 elements go into a launch; codes and scales behind them against the same in a small buffer"""
+    n, split = (1 << 33) + 1152, 1 << 33
+    if torch.cuda.mem_get_info()[0] < 12 * n:
+        pytest.skip("needs 103 GB")
+    codes = [torch.zeros(n, dtype=torch.uint8, device=cuda()) for _ in range(2)]
+    scales = [torch.zeros(n // 128, dtype=torch.uint8, device=cuda()) for _ in range(2)]
+    out = [torch.full((n,), 7.0, device=cuda()) for _ in range(2)]
+    places = [slice(0, 2048), slice(split - 2048, split), slice(split, n)]
+    gen = torch.Generator(cuda()).manual_seed(5)
+    for w in places:
+        for c, s in zip(codes, scales):
+            c[w] = torch.randint(0, 127, (w.stop - w.start,), generator=gen, device=cuda(), dtype=torch.uint8)
+            s[w.start // 128:w.stop // 128] = torch.randint(90, 140, ((w.stop - w.start) // 128,), generator=gen, device=cuda(), dtype=torch.uint8)
+
+    def decode(c, s, o):
+        rc = load_library().pinn_adamw_moments(*(t.data_ptr() for t in (*c, *s, *o)), o[0].numel(), _cur_stream(o[0]))
+        assert rc == 0
+    decode(codes, scales, out)
+    for w in places:
+        part = slice(w.start // 128, w.stop // 128)
+        want = [torch.full((w.stop - w.start,), 7.0, device=cuda()) for _ in range(2)]
+        decode([c[w].clone() for c in codes], [s[part].clone() for s in scales], want)
+        for o, x in zip(out, want):
+            assert torch.equal(o[w], x) and x.any()
+    assert all(float(o[split // 2:split // 2 + 4096].abs().max()) == 0.0 for o in out)
+    del codes, scales, out
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("dtype,bits", [(torch.float32, 32), (torch.bfloat16, 8)])
