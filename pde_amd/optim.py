@@ -173,6 +173,28 @@ def _partials(n, device):
     return torch.empty(room, dtype=torch.float64, device=device), room
 
 
+class _Place:
+    """where a tensor's elements lie, as numpy is told it: nothing is read"""
+
+    def __init__(self, t):
+        size = t.element_size()
+        self.__array_interface__ = dict(version=3, shape=tuple(t.shape), typestr="<i%d" % size, data=(t.data_ptr(), True),
+                                        strides=tuple(size * st for st in t.stride()))
+
+
+def _share_memory(tensors):
+    """Do two of the tensors have an element in common?  Exact for any strides: gradients may lie between each other's elements."""
+    places = sorted((np.asarray(_Place(t)) for t in tensors if t.numel()), key=lambda a: np.lib.array_utils.byte_bounds(a)[0])
+    ends = [np.lib.array_utils.byte_bounds(a) for a in places]
+    for i, a in enumerate(places):
+        for j in range(i + 1, len(places)):
+            if ends[j][0] >= ends[i][1]:
+                break
+            if np.shares_memory(a, places[j]):
+                return True
+    return False
+
+
 def _runs(rows, numel, chunk):
     """`rows`, tensors of `numel` elements, cut into what one launch of the step takes"""
     runs, chunks = [], 0
@@ -186,6 +208,9 @@ def _runs(rows, numel, chunk):
         runs[-1].append(i)
         chunks += more
     return runs
+
+
+_SHARED = "two of the gradients share memory: scaling them in place would scale it twice"
 
 
 def _as_list(tensors):
@@ -220,6 +245,9 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
         return torch.tensor(0.0)
     if any(0 in (st for sz, st in zip(g.shape, g.stride()) if sz > 1) for g, _ in lst.back):
         raise ValueError("a gradient that was expanded cannot be scaled in place")
+    # the C entry compares the memory that it scales; of these that is a copy
+    if lst.back and _share_memory([p.grad for p in parameters if p.grad is not None]):
+        raise ValueError(_SHARED)
     norm = torch.empty((), dtype=torch.float32, device=lst.device)
     lib = load_library()
     with _on(lst.device):
@@ -230,7 +258,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
                 raise RuntimeError("the gradients' norm is %s: they were not clipped" % norm.item())
         rc = lib.pinn_grad_clip(*lst.args, max_norm, norm.data_ptr(), stream)
         if rc == ERR_OVERLAP:
-            raise ValueError("two of the gradients share memory: scaling them in place would scale it twice")
+            raise ValueError(_SHARED)
         _check(rc, "pinn_grad_clip")
         for g, c in lst.back:
             g.copy_(c)
@@ -412,15 +440,14 @@ class GroupedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         sd = dict(state_dict)
-        fused = sd.pop("fused", None)
-        if fused is not None:
-            if sorted(fused) != sorted(self._held()):
-                raise ValueError("GroupedAdamW.load_state_dict: the state has %s, expected %s" % (sorted(fused), sorted(self._held())))
-            for name in self._held():
-                dst, src = getattr(self, name), fused[name]
-                if src.shape != dst.shape or src.dtype != dst.dtype:
-                    raise ValueError("GroupedAdamW.load_state_dict: %s is %s %s, expected %s %s"
-                                     % (name, tuple(src.shape), src.dtype, tuple(dst.shape), dst.dtype))
+        fused = sd.pop("fused", {})                      # another optimizer's moments would be dropped without a word
+        if sorted(fused) != sorted(self._held()):
+            raise ValueError("GroupedAdamW.load_state_dict: the state has %s, expected %s" % (sorted(fused), sorted(self._held())))
+        for name in self._held():
+            dst, src = getattr(self, name), fused[name]
+            if src.shape != dst.shape or src.dtype != dst.dtype:
+                raise ValueError("GroupedAdamW.load_state_dict: %s is %s %s, expected %s %s"
+                                 % (name, tuple(src.shape), src.dtype, tuple(dst.shape), dst.dtype))
         super().load_state_dict(sd)
         first = 0
         for grp in self.param_groups:                   # torch has replaced the groups' dicts
@@ -428,9 +455,8 @@ class GroupedAdamW(torch.optim.Optimizer):
                 if first <= launch["rows"][0] < first + len(grp["params"]):
                     launch["grp"] = grp
             first += len(grp["params"])
-        if fused is not None:
-            for name in self._held():
-                getattr(self, name).copy_(fused[name])
+        for name in self._held():
+            getattr(self, name).copy_(fused[name])
 
     def step(self, closure=None):
         """One step of every parameter that has a gradient; `closure` is called first, as in torch, and its loss returned."""

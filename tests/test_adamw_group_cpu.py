@@ -9,7 +9,7 @@ import torch
 
 import adamw_formulas as F
 from pde_amd._native import LIB_PATH, ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_CHUNK_DTYPE, ADAMW_MAX_CHUNKS, ADAMW_MAX_TENSORS, ADAMW_TICKET_WORDS, NORM_SMALL_ELEMENTS, NORM_SMALL_TENSORS, NativeError, PinnAdamWGroup, load_library
-from pde_amd.optim import GroupedAdamW, _runs, clip_grad_norm_, grad_norm
+from pde_amd.optim import GroupedAdamW, _runs, _share_memory, clip_grad_norm_, grad_norm
 from conftest import GOLDEN, ROOT
 
 needs_lib = pytest.mark.skipif(not os.path.exists(LIB_PATH), reason="libpinnjet.so not built")
@@ -137,6 +137,21 @@ def test_c_entries_refuse_without_a_gpu():
     assert clip(x=(ctypes.c_uint64 * 2)(4096, 4096 + 396)) == OVERLAP and clip(x=(ctypes.c_uint64 * 2)(8192, 8192)) == OVERLAP
     assert clip(x=(ctypes.c_uint64 * 2)(4096 + 396, 4096)) == OVERLAP
     assert lib.pinn_error_string(OVERLAP) == b"two tensors share memory"
+
+
+def test_shared_memory_of_any_strides():
+    """exact: columns that lie between each other's do not share, whatever their extents"""
+    a, b = torch.zeros(64, 6), torch.zeros(64, 6, dtype=torch.bfloat16)
+    flat = torch.zeros(100)
+    assert not _share_memory([])
+    assert not _share_memory([a, b, flat, torch.zeros(0), torch.tensor(1.0)])
+    assert not _share_memory([a[:, 0], a[:, 1], a[:, 2:4], a[:, 5], b[::2], b[1::2]])
+    assert not _share_memory([a.t()[4], a[:, 3], flat[:50], flat[50:], a[:0]])
+    assert _share_memory([flat, b[:, 0], b[:, 0]]) and _share_memory([a[:, 1:3], a[:, 2]]) and _share_memory([a[7], b, a[:, 5]])
+    assert _share_memory([flat[::2], flat[3::4], flat[2:3]])
+    assert not _share_memory([flat[::2], flat[3::4], flat[1:2]])
+    whole = torch.zeros(32, dtype=torch.float32)
+    assert _share_memory([whole, whole.view(torch.bfloat16)[::2][3:4]])
 
 
 def test_what_a_launch_takes():

@@ -462,6 +462,9 @@ def test_state_dict_continues(bits):
     other = GroupedAdamW(model(), state_bits=40 - bits, master_weights=True)
     with pytest.raises(ValueError, match="expected"):
         other.load_state_dict(a.state_dict())
+    for foreign in (torch.optim.AdamW(model()).state_dict(), {k: v for k, v in a.state_dict().items() if k != "fused"}):
+        with pytest.raises(ValueError, match="expected"):
+            other.load_state_dict(foreign)
     short = GroupedAdamW(params_of(make(SIZES[:-1], torch.float16, 70)), **kw)
     with pytest.raises(ValueError):
         short.load_state_dict(a.state_dict())
@@ -683,6 +686,18 @@ def test_refusals():
     with pytest.raises(ValueError, match="share memory"):
         clip_grad_norm_(p, 1e-3)
     assert torch.equal(kept, p[0].grad)
+    wide = make([(100, 3)], torch.float32, 122)[0]
+    before, lone = wide.clone(), p[1]
+    for one, two in ((wide[:, 0], wide[:, 0]), (wide[:, 1], wide.view(-1)[1:101])):
+        p[0].grad, lone.grad = one, two
+        with pytest.raises(ValueError, match="share memory"):
+            clip_grad_norm_(p, 1e-3)
+        assert torch.equal(wide, before)
+    p[0].grad, lone.grad = wide[:, 0], wide[:, 2]                                # between each other's elements: apart
+    norm = float(clip_grad_norm_(p, 1e-3))
+    assert abs(norm / float(before[:, ::2].norm()) - 1) < 1e-5 and torch.equal(wide[:, 1], before[:, 1])
+    assert (wide[:, ::2] - before[:, ::2] * (1e-3 / norm)).abs().max() < 1e-8
+    p[0].grad = p[1].grad = kept
     assert abs(float(grad_norm([p[0].grad, p[1].grad])) / (2 ** 0.5 * float(grad_norm(kept))) - 1) < 1e-6   # reading the same one twice is fine
     q = torch.nn.Parameter(torch.ones(4, 3, device=cuda()))
     q.grad = torch.ones(3, device=cuda()).expand(4, 3)
