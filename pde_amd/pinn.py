@@ -832,15 +832,21 @@ class PhysicsInformedNN:
         models and their graphs come and go; not reproduced, cause not established).  Two precautions: the cyclic
         garbage collector is paused for the duration, so that no older graph is destroyed and no device memory freed
         inside the capture, and an invalidated capture is attempted once more before the error is raised — nothing
-        that was captured has run."""
+        that was captured has run.
+
+        Where torch.distributed is initialised the capture is "thread_local": a process group's watchdog thread queries
+        the events of collectives that were eager shortly before, every 100 ms, and during a "global" capture that call is
+        an error in every thread of the process (hipErrorStreamCaptureUnsupported, which ends the process from there)."""
         import gc
+        import torch.distributed as dist
+        mode = "thread_local" if dist.is_available() and dist.is_initialized() else "global"
         last = None
         for _ in range(2):
             graph = torch.cuda.CUDAGraph()
             was_enabled = gc.isenabled()              # (torch.cuda.graph's __enter__ runs a full collection itself)
             gc.disable()
             try:
-                with torch.cuda.graph(graph):
+                with torch.cuda.graph(graph, capture_error_mode=mode):
                     out = body()
                 return graph, out
             except Exception as ex:                     # noqa: BLE001
