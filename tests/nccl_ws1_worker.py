@@ -96,7 +96,7 @@ def main():
         for p in ms.dnn.parameters():
             p.grad = None
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):   # the process group's watchdog queries events meanwhile
             terms = ms._loss_terms_sharded()
         graph.replay()
         torch.cuda.synchronize()
