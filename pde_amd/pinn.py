@@ -828,7 +828,7 @@ class PhysicsInformedNN:
 
     def _capture(self, body):
         """`body()` captured into a HIP graph: (graph, what body returned).  A capture can be invalidated by work that
-        is not its own (hipErrorStreamCaptureInvalidated was seen once in this round's GPU test runs, in a process where
+        is not its own (hipErrorStreamCaptureInvalidated was seen once in a GPU test run, in a process where
         models and their graphs come and go; not reproduced, cause not established).  Two precautions: the cyclic
         garbage collector is paused for the duration, so that no older graph is destroyed and no device memory freed
         inside the capture, and an invalidated capture is attempted once more before the error is raised — nothing
