@@ -86,12 +86,13 @@ __device__ inline void store_some(T *p, Vec<T, N> x, int have)
         if (e < have) p[e] = x[e];
 }
 
-// float32 rounded once to T.  The empty asm keeps the compiler from folding a float16 conversion into the fma before it
-// (v_fma_mixlo_f16 rounds the unrounded sum): a 16-bit weight is its float32 master's rounding, bit for bit.
+// float32 rounded once to T.  The empty asm keeps the compiler from folding the conversion into what comes before it
+// (v_fma_mixlo_f16 rounds the unrounded sum, and float64 by way of float32 becomes one conversion): a 16-bit weight is its
+// float32 master's rounding, bit for bit.
 template <class T>
 __device__ inline T rounded(float x)
 {
-    if constexpr (__is_same(T, _Float16)) asm("" : "+v"(x));
+    if constexpr (!__is_same(T, float)) asm("" : "+v"(x));
     return (T)x;
 }
 
@@ -111,8 +112,8 @@ struct StepConst {
     float *norm_out;
     int64_t n_chunks;
     int32_t n_tensors, n_partials, skip_nonfinite, run;
-    double max_norm, b1, b2, lr;
-    float eps, decay;
+    double max_norm, b1, b2, lr, eps, decay;
+    float eps32, decay32;
 };
 static_assert(sizeof(StepArgs) + sizeof(StepConst) <= 4096, "a launch's arguments");
 
@@ -138,28 +139,36 @@ __device__ inline double clip_factor(double norm, double max_norm)
 }
 
 // ---- float32 moments -------------------------------------------------------------------------------------------
+template <class F>
 struct Scalars {
-    float step_size, inv_bc2_sqrt;
+    F step_size, inv_bc2_sqrt;                  // float for float32 moments, double for 8 bits
     double p1, p2;
     uint32_t t;
 };
 
-// v_rcp_f64 and v_sqrt_f64 are good to about 2^-25; one Newton step gives the reciprocal twice the digits.  A full division and
-// root are 60 instructions, which a workgroup of 2048 elements feels.
+// v_rcp_f64 and v_rsq_f64 are good to 2^-23 at least; one Newton step gives them twice the digits.  A full division and root
+// are 60 instructions, which a workgroup of 2048 elements feels.
 __device__ inline double reciprocal(double x)
 {
     const double r = __builtin_amdgcn_rcp(x);
     return fma(r, fma(-x, r, 1.0), r);
 }
 
-__device__ inline Scalars scalars_of(const double *row, double b1, double b2, double lr)
+__device__ inline double reciprocal_root(double x)
 {
-    Scalars s;
+    const double r = __builtin_amdgcn_rsq(x);
+    return fma(0.5 * r, fma(-x * r, r, 1.0), r);
+}
+
+template <class F>
+__device__ inline Scalars<F> scalars_of(const double *row, double b1, double b2, double lr)
+{
+    Scalars<F> s;
     s.t = (uint32_t)(row[0] + 1.0);
     s.p1 = row[1] * b1;
     s.p2 = row[2] * b2;
-    s.step_size = (float)(lr * reciprocal(1.0 - s.p1));
-    s.inv_bc2_sqrt = (float)reciprocal(__builtin_amdgcn_sqrt(1.0 - s.p2));
+    s.step_size = (F)(lr * reciprocal(1.0 - s.p1));
+    s.inv_bc2_sqrt = (F)reciprocal_root(1.0 - s.p2);
     return s;
 }
 
@@ -167,7 +176,7 @@ struct Hyper32 {
     float b2, omb1, omb2, eps, decay, factor;
 };
 
-__device__ inline void update32(float &p, float g, float &m, float &v, const Scalars &s, const Hyper32 &h)
+__device__ inline void update32(float &p, float g, float &m, float &v, const Scalars<float> &s, const Hyper32 &h)
 {
     g *= h.factor;
     p *= h.decay;
@@ -190,7 +199,7 @@ struct At {
 };
 
 template <bool FULL, bool MASTER, class T>
-__device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper32 &h)
+__device__ inline void chunk(const At<T> &at, const Scalars<float> &s, const Hyper32 &h)
 {
     constexpr int N = 4;
     float *am = (float *)at.m, *av = (float *)at.v;
@@ -276,7 +285,7 @@ constexpr uint32_t kPlaceM = 0x9E3779B9u, kStepM = 0xC13FA9A9u, kPlaceV = 0x6A09
 
 struct Hyper8 {
     double b1, b2, g1, g2;                      // g1 = (1 - b1) f, g2 = (1 - b2) f^2
-    float eps, decay;
+    double eps, decay;
 };
 
 // a b + c d with each operation rounded by itself.  Codes are compared with where the remainder lies, and (9 m + g) / 10 lies on such a
@@ -309,7 +318,7 @@ __device__ inline void store_runs(T *p, Vec<T, 8> x, int have)
 }
 
 template <bool FULL, bool MASTER, class T>
-__device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper8 &h)
+__device__ inline void chunk(const At<T> &at, const Scalars<double> &s, const Hyper8 &h)
 {
     constexpr int N = 8, APART = sizeof(T) == 4 || MASTER ? kBlock / 2 : 4;
     const int lane = (int)threadIdx.x & 15, blk = (int)threadIdx.x >> 4;    // a block is 16 lanes, a DPP row
@@ -336,6 +345,9 @@ __device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper8 &h)
     if (s0m == 255) um = __hiloint2double(0x7ff80000, 0);
     if (s0v == 255) uv = __hiloint2double(0x7ff80000, 0);
     asm("" : "+v"(um), "+v"(uv));               // or the compiler makes the NaN a choice behind every product
+    // both terms of the denominator over the step size: the update is one product
+    const double per_step = s.step_size == 0.0 ? 1e300 : reciprocal(s.step_size), root = s.inv_bc2_sqrt * per_step, eps = h.eps * per_step;
+    const float decay32 = (float)h.decay;
     double md[N], vd[N];
     uint32_t hm = 0, hv = 0;
 #pragma unroll
@@ -350,9 +362,14 @@ __device__ inline void chunk(const At<T> &at, const Scalars &s, const Hyper8 &h)
         const uint32_t am = (uint32_t)__double2hiint(md[e]) & 0x7fffffffu, av = (uint32_t)__double2hiint(vd[e]);
         hm = am > hm ? am : hm;
         hv = av > hv ? av : hv;
-        // v_sqrt_f64 is good to 2^-25 over all of float64, v_rcp_f32 to 2^-23: beside the weight's own rounding they do not show
-        const float denom = fmaf((float)__builtin_amdgcn_sqrt(vd[e]), s.inv_bc2_sqrt, h.eps);
-        const float we = fmaf(-s.step_size * (float)md[e], __builtin_amdgcn_rcpf(denom), (MASTER ? w[e] : (float)p[e]) * h.decay);
+        // The denominator may be anything that a root of g^2 is: in float32 v_rcp_f32 gives 0 for the largest and infinity for
+        // subnormals.  v_sqrt_f64 and v_rcp_f64 are good to 2^-23 of the update at least, which does not show beside the weight's own
+        // rounding.  float32 weights and masters are rounded once, from float64.  A 16-bit weight's rounding is 2^13 times as coarse
+        // or more and hides the two of float32 (240M bfloat16 weights, the step with its read-out: 840 us, in float64 to the end 892).
+        const double update = md[e] * __builtin_amdgcn_rcp(fma(__builtin_amdgcn_sqrt(vd[e]), root, eps));
+        float we;
+        if constexpr (sizeof(T) == 4 || MASTER) we = (float)fma((double)(MASTER ? w[e] : (float)p[e]), h.decay, -update);
+        else we = fmaf((float)p[e], decay32, (float)-update);
         w[e] = we;
         p[e] = rounded<T>(we);
     }
@@ -456,15 +473,16 @@ __global__ __launch_bounds__(kThreads, BITS == 32 ? 6 : 5) void k_adamw_group(co
     }
     Hyper32 h32;
     Hyper8 h8;
-    if constexpr (BITS == 32) h32 = {(float)c.b2, (float)(1.0 - c.b1), (float)(1.0 - c.b2), c.eps, c.decay, (float)factor};
+    if constexpr (BITS == 32) h32 = {(float)c.b2, (float)(1.0 - c.b1), (float)(1.0 - c.b2), c.eps32, c.decay32, (float)factor};
     else h8 = {c.b1, c.b2, (1.0 - c.b1) * factor, (1.0 - c.b2) * factor * factor, c.eps, c.decay};
-    Scalars s;
+    typedef std::conditional_t<BITS == 32, float, double> F;
+    Scalars<F> s;
     const double *row = nullptr;
     const int64_t first = (int64_t)blockIdx.x * c.run, end = first + c.run < c.n_chunks ? first + c.run : c.n_chunks;
     for (int64_t ch = first; ch < end; ++ch) {
         const At<T> at = locate<T>(a, c, ch, BITS);
         if (!at.g) continue;
-        if (at.row != row) s = scalars_of(at.row, c.b1, c.b2, c.lr);
+        if (at.row != row) s = scalars_of<F>(at.row, c.b1, c.b2, c.lr);
         row = at.row;
         if constexpr (BITS == 32) {
             if (at.count == kChunk32) chunk<true, MASTER>(at, s, h32);
@@ -499,7 +517,7 @@ __global__ __launch_bounds__(kThreads, BITS == 32 ? 6 : 5) void k_adamw_group(co
     for (int k = threadIdx.x; k < c.n_tensors; k += kThreads)
         if (a.g[k]) {
             double *row = c.state + 3 * (int64_t)c.rows[k];
-            const Scalars n = scalars_of(row, c.b1, c.b2, c.lr);
+            const Scalars<F> n = scalars_of<F>(row, c.b1, c.b2, c.lr);
             row[0] += 1.0;
             row[1] = n.p1;
             row[2] = n.p2;
@@ -926,8 +944,10 @@ extern "C" int pinn_adamw_group_step(const PinnAdamWGroup *d, void *const *param
     c.b1 = d->beta1;
     c.b2 = d->beta2;
     c.lr = d->lr;
-    c.eps = (float)d->eps;
-    c.decay = (float)(1.0 - d->lr * d->weight_decay);
+    c.eps = d->eps;
+    c.decay = 1.0 - d->lr * d->weight_decay;
+    c.eps32 = (float)c.eps;
+    c.decay32 = (float)c.decay;
     const hipStream_t st = (hipStream_t)stream;
     if (d->dtype == PINN_F32) launch_step<float, false>(a, c, d->state_bits, st);
     else if (d->dtype == PINN_BF16) {

@@ -1,0 +1,72 @@
+"""GPU: GroupedAdamW, grad_norm and clip_grad_norm_ at the ends of float32's range and around captured calls, against float64 numpy
+(adamw_formulas.py).  h = 2^-24 is the half step of float32."""
+import numpy as np
+import pytest
+import torch
+
+import adamw_formulas as F
+from pde_amd._native import NORM_SMALL_ELEMENTS
+from pde_amd.optim import GroupedAdamW, clip_grad_norm_, grad_norm
+
+pytestmark = pytest.mark.gpu
+H = 2.0 ** -24
+
+
+def cuda():
+    return torch.device("cuda", 0)
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy().reshape(-1)
+
+
+def on_gpu(x, dtype=torch.float32):
+    return torch.tensor(np.asarray(x), dtype=torch.float32).to(dtype).to(cuda())
+
+
+# ---- the weights' update with 8-bit moments ------------------------------------------------------------------------
+@pytest.mark.parametrize("lo,hi,eps", [(1e38, 3e38, 1e-8), (1e37, 1e38, 0.0), (1e-40, 1e-38, 0.0), (1e-44, 1e-42, 0.0), (1e-40, 1e-38, 1e-39)])
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, False), (torch.bfloat16, True)])
+def test_eight_bit_update_over_the_range(dtype, master, lo, hi, eps):
+    """The first step moves a weight by lr |m^| / (sqrt(v^) + eps), lr where eps is nothing beside the gradient, however large or small that is:
+    the denominator passes 2^126 above and float32's subnormals below.  At most 16 roundings of the update (half a step of a 16-bit weight more)."""
+    rng = np.random.default_rng(1)
+    n, lr = 1000, 1e-2
+    g = on_gpu(rng.uniform(lo, hi, n) * rng.choice([-1.0, 1.0], n), dtype)
+    p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=cuda()))
+    p.grad = g
+    opt = GroupedAdamW([p], lr=lr, eps=eps, weight_decay=0.0, state_bits=8, master_weights=master)
+    opt.step()
+    p1, _, _ = F.step(np.zeros(n), f64(g), np.zeros(n), np.zeros(n), 1, lr, 0.9, 0.999, eps, 0.0)
+    # a gradient that its type rounds to 0 is 0 / 0 where eps is 0
+    zero = f64(g) == 0.0
+    assert zero.all() == (dtype != torch.float32 and hi < 1e-41) and np.array_equal(np.isnan(p1), zero) and np.array_equal(np.isnan(f64(p)), zero)
+    half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+    assert (np.abs(f64(p) - p1) <= (16 * H + half) * np.abs(p1))[~zero].all()
+
+
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, True), (torch.float16, True)])
+def test_eight_bit_step_rounds_float32_weights_once(dtype, master):
+    """The sum (1 - lr wd) p - U is formed in float64 and rounded to float32 once: half a step of the result.  U has the two approximations of
+    its root and its reciprocal, each within 2^29 of float64's last places (2^-23 of the value), and nothing else that counts."""
+    rng = np.random.default_rng(2)
+    sizes, lr, wd = [5000, 127, 2049], 1e-3, 1e-2
+    params = [torch.nn.Parameter(on_gpu(0.1 * rng.standard_normal(n), dtype)) for n in sizes]
+    opt = GroupedAdamW(params, lr=lr, weight_decay=wd, state_bits=8, master_weights=master, max_norm=3.0)
+
+    def weights(i):
+        return f64(opt.master[opt.offsets[i]:opt.offsets[i] + sizes[i]] if master else params[i])
+    for t in range(1, 5):
+        for p in params:
+            p.grad = on_gpu(rng.standard_normal(p.numel()), dtype)
+        ms, vs = (f64(x) for x in opt.moments())
+        had = [weights(i) for i in range(len(sizes))]
+        grads = [f64(p.grad) for p in params]
+        _, factor = F.clip_factor(grads, 3.0)
+        opt.step()
+        for i, n in enumerate(sizes):
+            at = slice(opt.offsets[i], opt.offsets[i] + n)
+            p1, _, _ = F.step(had[i], grads[i] * factor, ms[at], vs[at], t, lr, 0.9, 0.999, 1e-8, wd)
+            update = np.abs(p1 - had[i] * (1 - lr * wd))
+            half = np.spacing(np.abs(p1).astype(np.float32)).astype(np.float64) / 2
+            assert (np.abs(weights(i) - p1) <= half * (1 + 1e-6) + 2.0 ** -22 * update).all(), (t, i)
