@@ -220,7 +220,7 @@ def _as_list(tensors):
 def grad_norm(tensors):
     """2-norm over all elements of all `tensors` (one, or an iterable; float32, bfloat16, float16, mixed as they come): a 0-dim
     float32 tensor on their device.  Squares and sums are float64, in a fixed order: the same inputs give the same bits, and
-    no float32 value overflows or vanishes on the way.  An empty list gives 0."""
+    no float32 value overflows or vanishes on the way (a norm beyond float32's largest value reads infinity).  An empty list gives 0."""
     tensors = _as_list(tensors)
     if not tensors:
         return torch.tensor(0.0)
@@ -235,7 +235,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     """Scales the gradients of `parameters` in place so that their global 2-norm is at most `max_norm`, and returns the norm
     they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 250 tensors (one for few elements),
     without a copy of the gradients.  The factor is min(1, max_norm / (norm + 1e-6)); with a norm that is not finite it is 0 or NaN, as
-    there; `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError)."""
+    there (the factor goes by the float64 norm, also where the one returned is beyond float32 and reads infinity); `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError)."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm is %r: 0 or more is needed" % max_norm)

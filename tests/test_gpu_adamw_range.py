@@ -70,3 +70,45 @@ def test_eight_bit_step_rounds_float32_weights_once(dtype, master):
             update = np.abs(p1 - had[i] * (1 - lr * wd))
             half = np.spacing(np.abs(p1).astype(np.float32)).astype(np.float64) / 2
             assert (np.abs(weights(i) - p1) <= half * (1 + 1e-6) + 2.0 ** -22 * update).all(), (t, i)
+
+
+# ---- norms beyond float32 ------------------------------------------------------------------------------------------
+def huge(n, dtype, seed):
+    rng = np.random.default_rng(seed)
+    return on_gpu(rng.uniform(1e38, 3e38, n) * rng.choice([-1.0, 1.0], n), dtype)
+
+
+@pytest.mark.parametrize("max_norm", [1.0, 1e-20, 1e30])
+@pytest.mark.parametrize("n", [1000, 100000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clipping_of_a_norm_beyond_float32(dtype, n, max_norm):
+    """The norm reads infinity there, the factor comes from its float64 value (1e-40 and less: not a float32 with 24 bits), which is rounded once as is
+    the product: h each, and half a step of bfloat16"""
+    p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=cuda()))
+    p.grad = huge(n, dtype, 3)
+    g = f64(p.grad)
+    norm, factor = F.clip_factor([g], max_norm)
+    assert norm > torch.finfo(torch.float32).max and factor < 1e-7
+    assert float(clip_grad_norm_(p, max_norm)) == float("inf")
+    want = g * factor
+    assert (np.abs(f64(p.grad) - want) <= 2 * H * np.abs(want) + (torch.finfo(dtype).eps / 2 * np.abs(want) if dtype != torch.float32 else 0.0)).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_step_clipped_from_a_norm_beyond_float32(dtype, bits):
+    """first moments after one step: the tolerance of test_gpu_adamw_group.py, 8-bit codes equal"""
+    n = 3000
+    p = torch.nn.Parameter(torch.zeros(n, dtype=dtype, device=cuda()))
+    p.grad = huge(n, dtype, 4)
+    opt = GroupedAdamW([p], state_bits=bits, max_norm=1.0)
+    opt.step()
+    g = f64(p.grad)
+    _, factor = F.clip_factor([g], 1.0)
+    _, m1, v1 = F.step(np.zeros(n), g * factor, np.zeros(n), np.zeros(n), 1)
+    m, v = (f64(x)[:n] for x in opt.moments())
+    assert float(opt.grad_norm) == float("inf") and opt.device_state[0, 0] == 1.0
+    if bits == 8:
+        assert np.array_equal(m, F.round_flat(m1, 0, 1, F.M)[0]) and np.array_equal(v, F.round_flat(v1, 0, 1, F.V)[0])
+    else:
+        assert (np.abs(m - m1) <= H * (np.abs(m1) + 0.4 * np.abs(g * factor))).all() and (np.abs(v - v1) <= 8 * H * v1).all()
