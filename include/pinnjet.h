@@ -298,7 +298,7 @@ typedef struct {
     int32_t n_tensors;
     int32_t dtype;                   /* of parameters and gradients */
     int32_t state_bits;              /* 32 or 8 */
-    int32_t skip_nonfinite;          /* with partials: a norm that is not finite leaves everything as it was */
+    int32_t skip_nonfinite;          /* with partials: a norm that is not finite, as a float32, leaves everything as it was */
     void *exp_avg, *exp_avg_sq;      /* float32, or codes */
     uint8_t *exp_avg_scale, *exp_avg_sq_scale;
     float *master;                   /* NULL: none; else the weights that are updated, the parameters are their rounded copy */

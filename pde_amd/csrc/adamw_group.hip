@@ -486,7 +486,7 @@ __global__ __launch_bounds__(kThreads, BITS == 32 ? 6 : 5) void k_adamw_group(co
     if (c.n_partials) {
         const double norm = sqrt(sum_partials(c.partials, c.n_partials));
         if (c.norm_out && blockIdx.x == 0 && threadIdx.x == 0) *c.norm_out = (float)norm;
-        if (c.skip_nonfinite && !(norm < __hiloint2double(0x7ff00000, 0))) return;   // in all workgroups alike: nothing is written, the tickets stay
+        if (c.skip_nonfinite && !((float)norm < __uint_as_float(0x7f800000u))) return;   // as it is reported; in all workgroups alike: nothing is written, the tickets stay
         if (c.max_norm >= 0.0) factor = clip_factor(norm, c.max_norm);
     }
     const Hyper32 h32 = {(float)c.b2, (float)(1.0 - c.b1), (float)(1.0 - c.b2), c.eps32, c.decay32, Factor(factor)};

@@ -276,7 +276,7 @@ class GroupedAdamW(torch.optim.Optimizer):
                     rounded by an even sequence, so that small changes are not lost.  A gradient that is not finite makes its whole block's moments NaN.
     max_norm        clip the gradients' global 2-norm (over all groups, tensors without a gradient left out) inside the step; the gradients themselves
                     stay as they are.  `grad_norm` holds the norm of the last step, on the device.
-    skip_nonfinite  a step whose gradient norm is not finite changes nothing, counters included (decided on the device).
+    skip_nonfinite  a step whose gradient norm is not finite, as `grad_norm` gives it, changes nothing, counters included (decided on the device).
     master_weights  bfloat16 and float16 parameters are the rounded copy of float32 weights held here (`master`); after writing to
                     such a parameter from outside call `sync_master()`.
 

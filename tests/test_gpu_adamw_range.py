@@ -112,3 +112,17 @@ def test_step_clipped_from_a_norm_beyond_float32(dtype, bits):
         assert np.array_equal(m, F.round_flat(m1, 0, 1, F.M)[0]) and np.array_equal(v, F.round_flat(v1, 0, 1, F.V)[0])
     else:
         assert (np.abs(m - m1) <= H * (np.abs(m1) + 0.4 * np.abs(g * factor))).all() and (np.abs(v - v1) <= 8 * H * v1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_skip_goes_by_the_norm_that_is_reported(bits):
+    p = torch.nn.Parameter(on_gpu(np.ones(2000)))
+    p.grad = huge(2000, torch.float32, 5)
+    opt = GroupedAdamW([p], state_bits=bits, skip_nonfinite=True)
+    before = opt.state_dict()["fused"]
+    opt.step()
+    after = opt.state_dict()["fused"]
+    assert float(opt.grad_norm) == float("inf") and (p == 1).all() and all(torch.equal(before[k], after[k]) for k in after)
+    p.grad.mul_(1e-10)
+    opt.step()
+    assert torch.isfinite(opt.grad_norm) and opt.device_state[0, 0] == 1.0 and not (p == 1).any()
