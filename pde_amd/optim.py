@@ -412,7 +412,7 @@ class GroupedAdamW(torch.optim.Optimizer):
 
     @property
     def grad_norm(self):
-        """norm of the gradients of the last step (0-dim float32, overwritten by the next); steps without `max_norm` or `skip_nonfinite` do not form it"""
+        """norm of the gradients of the last step (0-dim float32, overwritten by the next; 0 where no parameter had one); steps without `max_norm` or `skip_nonfinite` do not form it"""
         return self._norm
 
     def moments(self):
@@ -480,7 +480,10 @@ class GroupedAdamW(torch.optim.Optimizer):
             self._p[0], first = 0, self._p[0]           # found wanting, they are looked at again in the next step
             self._check_params()
             self._p[0] = first
+        clipped = self.max_norm is not None or self.skip_nonfinite
         if not given:
+            if clipped:
+                self._norm.zero_()                      # the norm of no gradients, not the last step's
             return loss
         keep = []
         for i in other:                                 # a gradient in another order in memory than its parameter
@@ -490,7 +493,7 @@ class GroupedAdamW(torch.optim.Optimizer):
         with _on(self.device):
             stream = _cur_stream(self._norm)
             partials, n_partials = None, 0
-            if self.max_norm is not None or self.skip_nonfinite:
+            if clipped:
                 partials, room = _partials(len(self._ordered), self.device)
                 found = ctypes.c_int32()
                 _check(self.lib.pinn_grad_sumsq(self._g, self._count, self._dtype, len(self._ordered), partials.data_ptr(), room,

@@ -126,3 +126,17 @@ def test_skip_goes_by_the_norm_that_is_reported(bits):
     p.grad.mul_(1e-10)
     opt.step()
     assert torch.isfinite(opt.grad_norm) and opt.device_state[0, 0] == 1.0 and not (p == 1).any()
+
+
+# ---- what a step without gradients reports ---------------------------------------------------------------------------
+@pytest.mark.parametrize("options", [dict(max_norm=1.0), dict(skip_nonfinite=True)])
+def test_norm_of_a_step_without_gradients(options):
+    p = torch.nn.Parameter(on_gpu(np.ones(50)))
+    opt = GroupedAdamW([p], **options)
+    p.grad = on_gpu(np.full(50, 2.0))
+    opt.step()
+    assert abs(float(opt.grad_norm) / (2.0 * 50 ** 0.5) - 1) < 1e-6
+    after = p.detach().clone()
+    opt.zero_grad()
+    opt.step()
+    assert float(opt.grad_norm) == 0.0 and torch.equal(p, after) and opt.device_state[0, 0] == 1.0
