@@ -235,7 +235,11 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     """Scales the gradients of `parameters` in place so that their global 2-norm is at most `max_norm`, and returns the norm
     they had (0-dim float32, on the device): torch.nn.utils.clip_grad_norm_ in two launches per 250 tensors (one for few elements),
     without a copy of the gradients.  The factor is min(1, max_norm / (norm + 1e-6)); with a norm that is not finite it is 0 or NaN, as
-    there (the factor goes by the float64 norm, also where the one returned is beyond float32 and reads infinity); `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError)."""
+    there (the factor goes by the float64 norm, also where the one returned is beyond float32 and reads infinity);
+    `error_if_nonfinite` raises instead and waits for the GPU.  Gradients that share memory are refused (ValueError), and so is
+    a third argument that is not a truth value (TypeError): there is no `norm_type`."""
+    if not isinstance(error_if_nonfinite, (bool, np.bool_)):
+        raise TypeError("error_if_nonfinite is %r: True or False is needed (the norm is always the 2-norm)" % (error_if_nonfinite,))
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError("max_norm is %r: 0 or more is needed" % max_norm)
