@@ -305,6 +305,8 @@ class GroupedAdamW(torch.optim.Optimizer):
             self._hyper(grp)
         self._chunk = ADAMW_CHUNK32 if state_bits == 32 else ADAMW_CHUNK8
         self._params = [p for grp in self.param_groups for p in grp["params"]]
+        if not self._params:
+            raise ValueError("the groups have no parameter")
         self.device = self._params[0].device
         if self.device.type != "cuda":
             raise NativeError("GroupedAdamW needs parameters on an AMD GPU, got %s; there is no CPU fallback (use torch.optim.AdamW)" % self.device)

@@ -14,3 +14,8 @@ def test_a_norm_type_is_not_taken_for_error_if_nonfinite(third):
     with pytest.raises(TypeError, match="2-norm"):
         clip_grad_norm_([p], 1.0, third)
     assert torch.equal(p.grad, torch.ones(3))
+
+
+def test_groups_without_any_parameter_are_refused():
+    with pytest.raises(ValueError, match="no parameter"):
+        GroupedAdamW([dict(params=[]), dict(params=[])])
