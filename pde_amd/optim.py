@@ -11,6 +11,7 @@ weights, moments in 32 or 8 bits, clipping of the global gradient norm; `grad_no
 
 There is no CPU fallback: all of it needs libpinnjet.so and a GPU.
 """
+import bisect
 import ctypes
 
 import numpy as np
@@ -178,20 +179,47 @@ class _Place:
 
     def __init__(self, t):
         size = t.element_size()
-        self.__array_interface__ = dict(version=3, shape=tuple(t.shape), typestr="<i%d" % size, data=(t.data_ptr(), True),
-                                        strides=tuple(size * st for st in t.stride()))
+        self.begin = t.data_ptr()
+        self.end = self.begin + size * (1 + sum(st * (n - 1) for n, st in zip(t.shape, t.stride())))     # torch's strides are never negative
+        self.numel = t.numel()
+        self.strides = tuple(size * st for st in t.stride())
+        self.__array_interface__ = dict(version=3, shape=tuple(t.shape), typestr="<i%d" % size, data=(self.begin, True), strides=self.strides)
 
 
 def _share_memory(tensors):
     """Do two of the tensors have an element in common?  Exact for any strides: gradients may lie between each other's elements."""
-    places = sorted((np.asarray(_Place(t)) for t in tensors if t.numel()), key=lambda a: np.lib.array_utils.byte_bounds(a)[0])
-    ends = [np.lib.array_utils.byte_bounds(a) for a in places]
-    for i, a in enumerate(places):
-        for j in range(i + 1, len(places)):
-            if ends[j][0] >= ends[i][1]:
-                break
-            if np.shares_memory(a, places[j]):
+    places = sorted((_Place(t) for t in tensors if t.numel()), key=lambda p: p.begin)
+    first, end = 0, 0
+    for i, p in enumerate(places):                      # runs of tensors whose extents hang together
+        if p.begin >= end:
+            if _run_shares(places[first:i]):
                 return True
+            first = i
+        end = max(end, p.end)
+    return _run_shares(places[first:])
+
+
+def _run_shares(places):
+    """Two ways.  numpy compares two arrays in 0.7 us whatever their size (where their strides are simple: the search is cut off at
+    10^5 steps); marking every element takes about 20 ns for each.  512 columns of 100 elements: 90 ms by pairs, 4.8 by marks; 65 of 1000: 1.6 and
+    1.3; 2 of 10^7: 0.014 and 250."""
+    begins = [p.begin for p in places]
+    meets = [bisect.bisect_left(begins, p.end) for p in places]                     # the first behind those that begin before p ends
+    if 32 * sum(m - i - 1 for i, m in enumerate(meets)) <= sum(p.numel for p in places):
+        try:
+            arrays = [np.asarray(p) for p in places]
+            return any(np.shares_memory(a, b, max_work=100000) for i, a in enumerate(arrays) for b in arrays[i + 1:meets[i]])
+        except RuntimeError:                            # TooHardError
+            pass
+    if len(places) < 2:
+        return False
+    taken = np.zeros((max(p.end for p in places) - begins[0]) // 2, dtype=bool)     # two bytes each: a 16-bit element or half of another
+    for p in places:
+        a = np.asarray(p)
+        mine = np.ndarray(a.shape + (a.itemsize // 2,), bool, taken, (p.begin - begins[0]) // 2, tuple(st // 2 for st in p.strides) + (1,))
+        if mine.any():
+            return True
+        mine[...] = True
     return False
 
 
