@@ -332,6 +332,11 @@ int pinn_grad_clip(void *const *grads, const int64_t *numel, const int32_t *dtyp
 
 const char *pinn_error_string(int code);
 
+/* What a caller's structs and tables are laid out by, for one that was compiled apart from the library to compare: writes the first n of these
+ * and returns how many there are.  sizeof pinn_desc and for each of its fields the name's 32-bit FNV-1a hash and the offset, the same of PinnAdamWChunk and PinnAdamWGroup, then PINN_ADAMW_BLOCK,
+ * _CHUNK32, _CHUNK8, _MAX_TENSORS, _MAX_CHUNKS, _TICKET_WORDS, PINN_NORM_SMALL_TENSORS, _SMALL_ELEMENTS, PINN_ERR_OVERLAP. */
+int32_t pinn_layout(int32_t *out, int32_t n);
+
 #define PINN_OK 0
 #define PINN_ERR_INVALID_DESC (-1)
 #define PINN_ERR_UNSUPPORTED (-2)

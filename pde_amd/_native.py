@@ -65,7 +65,40 @@ SYMBOLS = [
     "pinn_lbfgs_direction_advance", "pinn_lbfgs_eval_stats_keep", "pinn_host_device_pointer",
     "pinn_lbfgs_poll_advance",
     "pinn_adamw_group_step", "pinn_adamw_moments", "pinn_grad_norm_partials", "pinn_grad_sumsq", "pinn_grad_norm", "pinn_grad_clip",
+    "pinn_layout",
 ]
+
+
+def _layout():
+    """what the structs and tables here are laid out by, in pinn_layout's order"""
+    def of(size, offsets):
+        out = [size]
+        for name, offset in offsets:
+            h = 2166136261
+            for c in name.encode():
+                h = (h ^ c) * 16777619 & 0xffffffff
+            out += [ctypes.c_int32(h).value, offset]
+        return out
+
+    def of_struct(s):
+        return of(ctypes.sizeof(s), [(name, getattr(s, name).offset) for name, _ in s._fields_])
+    chunk = of(ADAMW_CHUNK_DTYPE.itemsize, [(name, ADAMW_CHUNK_DTYPE.fields[name][1]) for name in ADAMW_CHUNK_DTYPE.names])
+    return of_struct(PinnDesc) + chunk + of_struct(PinnAdamWGroup) + [ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_MAX_TENSORS, ADAMW_MAX_CHUNKS, ADAMW_TICKET_WORDS,
+                                      NORM_SMALL_TENSORS, NORM_SMALL_ELEMENTS, ERR_OVERLAP]
+
+
+def _check_library(lib):
+    """A library of another build would take these structs for others and read past the tables."""
+    missing = [name for name in SYMBOLS if not hasattr(lib, name)]
+    found = None
+    if not missing:
+        lib.pinn_layout.argtypes = [ctypes.c_void_p, ctypes.c_int32]
+        theirs = (ctypes.c_int32 * lib.pinn_layout(None, 0))()
+        lib.pinn_layout(theirs, len(theirs))
+        found = list(theirs)
+    if found != _layout():
+        raise NativeError("%s is of another build than this package (%s): build it again with `python -c 'import __graft_entry__ as g; g.build()'`"
+                          % (LIB_PATH, "without " + ", ".join(missing) if missing else "structs or constants differ"))
 
 
 def load_library():
@@ -78,6 +111,7 @@ def load_library():
             "pde_amd/libpinnjet.so is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
             "(hipcc --offload-arch=gfx950).  There is no CPU fallback.")
     lib = ctypes.CDLL(LIB_PATH)
+    _check_library(lib)
     vp, i64, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
     lib.pinn_create.argtypes = [ctypes.POINTER(PinnDesc), ctypes.POINTER(vp)]
     lib.pinn_destroy.argtypes = [vp]

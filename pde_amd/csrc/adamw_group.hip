@@ -21,6 +21,7 @@
 // contracts a float32 expression.  240M weights: float32 660 us (16 bytes each, 5.8 TB/s), bfloat16 440 us (10 bytes, 5.5 TB/s: its 52
 // vector instructions an element, 360 us of issue, no longer hide under 387 us of memory).
 #include <hip/hip_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 #include <stdlib.h>
 
@@ -860,6 +861,37 @@ void fold(double *partials, int32_t &n_partials, void *stream)
 }
 
 }  // namespace
+
+// FNV-1a
+static constexpr int32_t name_hash(const char *s)
+{
+    uint32_t h = 2166136261u;
+    for (; *s; ++s) h = (h ^ (uint8_t)*s) * 16777619u;
+    return (int32_t)h;
+}
+
+extern "C" int32_t pinn_layout(int32_t *out, int32_t n)
+{
+#define AT(S, F) name_hash(#F), (int32_t)offsetof(S, F)
+#define CHUNK(F) AT(PinnAdamWChunk, F)
+#define GROUP(F) AT(PinnAdamWGroup, F)
+    static constexpr int32_t layout[] = {
+        (int32_t)sizeof(pinn_desc), AT(pinn_desc, eq), AT(pinn_desc, n_lin), AT(pinn_desc, widths), AT(pinn_desc, lb), AT(pinn_desc, ub),
+        AT(pinn_desc, coef), AT(pinn_desc, kernel), AT(pinn_desc, reserved),
+        (int32_t)sizeof(PinnAdamWChunk), CHUNK(base), CHUNK(place), CHUNK(count), CHUNK(tensor), CHUNK(row), CHUNK(reserved),
+        (int32_t)sizeof(PinnAdamWGroup), GROUP(chunks), GROUP(rows), GROUP(n_chunks), GROUP(n_tensors), GROUP(dtype), GROUP(state_bits),
+        GROUP(skip_nonfinite), GROUP(exp_avg), GROUP(exp_avg_sq), GROUP(exp_avg_scale), GROUP(exp_avg_sq_scale), GROUP(master),
+        GROUP(device_state), GROUP(ticket), GROUP(partials), GROUP(n_partials), GROUP(reserved), GROUP(norm), GROUP(max_norm), GROUP(lr),
+        GROUP(beta1), GROUP(beta2), GROUP(eps), GROUP(weight_decay),
+        PINN_ADAMW_BLOCK, PINN_ADAMW_CHUNK32, PINN_ADAMW_CHUNK8, PINN_ADAMW_MAX_TENSORS, PINN_ADAMW_MAX_CHUNKS, PINN_ADAMW_TICKET_WORDS,
+        PINN_NORM_SMALL_TENSORS, PINN_NORM_SMALL_ELEMENTS, PINN_ERR_OVERLAP};
+#undef GROUP
+#undef CHUNK
+#undef AT
+    const int32_t count = (int32_t)(sizeof(layout) / sizeof(layout[0]));
+    for (int32_t i = 0; out && i < n && i < count; ++i) out[i] = layout[i];
+    return count;
+}
 
 extern "C" int64_t pinn_grad_norm_partials(int32_t n_tensors)
 {

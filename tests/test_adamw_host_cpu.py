@@ -1,10 +1,15 @@
 """CPU: the host side of GroupedAdamW, grad_norm and clip_grad_norm_ - arguments that would be taken for others, parameter lists without
 a parameter, gradients that share memory, libraries that do not fit this package."""
+import os
+
 import numpy as np
 import pytest
 import torch
 
+from pde_amd import _native as native
 from pde_amd.optim import GroupedAdamW, _share_memory, clip_grad_norm_
+
+needs_lib = pytest.mark.skipif(not os.path.exists(native.LIB_PATH), reason="libpinnjet.so not built")
 
 
 @pytest.mark.parametrize("third", [2.0, 1.0, 2, 1, float("inf"), "inf", None])
@@ -76,3 +81,28 @@ def test_shared_memory_that_is_hard_to_decide():
     strides = [1009, 1013, 1019, 1021, 1031, 1033, 1039]
     a, b = base.as_strided([6] * 7, strides, 0), base.as_strided([6] * 7, [s + 2 for s in strides], 1)
     assert isinstance(_share_memory([a, b]), bool)
+
+
+@needs_lib
+def test_a_library_of_another_build_is_noticed(monkeypatch):
+    """its chunk size, the order or the size of the structs' fields, a missing entry point: it is not called"""
+    import ctypes
+
+    def loads():
+        monkeypatch.setattr(native, "_lib", None)
+        return native.load_library()
+    loads()
+
+    class Swapped(ctypes.Structure):
+        fields = list(native.PinnAdamWGroup._fields_)
+        i = [name for name, _ in fields].index("exp_avg")
+        fields[i], fields[i + 1] = fields[i + 1], fields[i]
+        _fields_ = fields
+    for name, value in (("ADAMW_CHUNK8", 4096), ("ADAMW_TICKET_WORDS", 1), ("PinnAdamWGroup", Swapped), ("SYMBOLS", native.SYMBOLS + ["pinn_not_there"]),
+                        ("ADAMW_CHUNK_DTYPE", np.dtype([("base", np.int64), ("place", np.int64), ("tensor", np.int32), ("count", np.int32),
+                                                        ("row", np.int32), ("reserved", np.int32)]))):
+        with monkeypatch.context() as m:
+            m.setattr(native, name, value)
+            with pytest.raises(native.NativeError, match="build it again"):
+                loads()
+    loads()
