@@ -1,0 +1,46 @@
+"""CPU: what build() takes for up to date."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+import __graft_entry__ as entry
+from conftest import ROOT
+
+
+def writes(out, text):
+    return [sys.executable, "-c", "import sys; open(sys.argv[1], 'w').write(sys.argv[2])", out, text]
+
+
+def test_objects_go_by_their_command_line_too(tmp_path):
+    src, out = tmp_path / "a.hip", str(tmp_path / "a.o")
+    src.write_text("x")
+    os.utime(src, (1, 1))
+    deps = [str(src)]
+    assert entry._compile(writes(out, "1"), out, deps, False)
+    assert not entry._compile(writes(out, "1"), out, deps, False)              # nothing has changed
+    assert entry._compile(writes(out, "1"), out, deps, True)                   # asked for
+    assert entry._compile(writes(out, "2"), out, deps, False) and open(out).read() == "2"     # another flag
+    os.utime(src)
+    os.utime(out, (2, 2))
+    assert entry._compile(writes(out, "2"), out, deps, False)                  # a newer source
+    os.remove(out + ".cmd")
+    assert entry._compile(writes(out, "2"), out, deps, False)                  # made before command lines were kept
+
+
+def test_a_failed_compile_leaves_nothing_older(tmp_path):
+    out = str(tmp_path / "a.o")
+    entry._compile(writes(out, "1"), out, [], True)
+    with pytest.raises(subprocess.CalledProcessError):
+        entry._compile([sys.executable, "-c", "raise SystemExit(1)"], out, [], True)
+    assert not os.path.exists(out) and not os.path.exists(out + ".cmd")
+
+
+def test_build_compiles_every_unit_every_time(monkeypatch):
+    ran = []
+    monkeypatch.setattr(entry, "_compile", lambda cmd, out, deps, force: ran.append((os.path.basename(out), force)))
+    monkeypatch.setattr(entry.subprocess, "check_call", lambda cmd: None)
+    entry.build()
+    units = [f + ".o" for f in os.listdir(os.path.join(ROOT, "pde_amd", "csrc")) if f.endswith(".hip")]
+    assert sorted(ran) == sorted((name, True) for name in units + ["libpinnjet.so", "_tensorlist.so"])
