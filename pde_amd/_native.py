@@ -153,14 +153,24 @@ def load_library():
     return lib
 
 
+_list = None
+
+
 def load_tensorlist():
-    """The in-tree extension module that reads lists of tensors (csrc/tensorlist.cpp); raises if it was not built."""
+    """The in-tree extension module that reads lists of tensors (csrc/tensorlist.cpp); raises if it was not built, or for another torch."""
+    global _list
+    if _list is not None:
+        return _list
     try:
         from . import _tensorlist
+        found = getattr(_tensorlist, "torch_version", "another torch")
+        if found != str(torch.__version__):
+            raise ImportError("for %s, this is %s" % (found, torch.__version__))
     except ImportError as ex:
         raise NativeError("pde_amd/_tensorlist.so is missing or was built for another torch (%s): build it with "
                           "`python -c 'import __graft_entry__ as g; g.build()'`" % ex) from ex
-    return _tensorlist
+    _list = _tensorlist
+    return _list
 
 
 def _check(rc, what):

@@ -194,4 +194,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensorlist", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensorlist() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__tensorlist()
+{
+    PyObject *m = PyModule_Create(&module);
+    // which torch's tensors this was compiled for: they are read by its headers
+    if (m && PyModule_AddStringConstant(m, "torch_version", PINN_TORCH) != 0) Py_CLEAR(m);
+    return m;
+}

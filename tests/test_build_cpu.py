@@ -1,11 +1,13 @@
-"""CPU: what build() takes for up to date."""
+"""CPU: what build() takes for up to date, and modules built for another torch."""
 import os
 import subprocess
 import sys
 
 import pytest
+import torch
 
 import __graft_entry__ as entry
+from pde_amd import _native as native
 from conftest import ROOT
 
 
@@ -44,3 +46,12 @@ def test_build_compiles_every_unit_every_time(monkeypatch):
     entry.build()
     units = [f + ".o" for f in os.listdir(os.path.join(ROOT, "pde_amd", "csrc")) if f.endswith(".hip")]
     assert sorted(ran) == sorted((name, True) for name in units + ["libpinnjet.so", "_tensorlist.so"])
+
+
+@pytest.mark.skipif(not os.path.exists(os.path.join(ROOT, "pde_amd", "_tensorlist.so")), reason="_tensorlist.so not built")
+def test_a_list_reader_for_another_torch_is_noticed(monkeypatch):
+    assert native.load_tensorlist().torch_version == str(torch.__version__)
+    monkeypatch.setattr(native, "_list", None)
+    monkeypatch.setattr(torch, "__version__", "2.0.0")
+    with pytest.raises(native.NativeError, match="another torch"):
+        native.load_tensorlist()
