@@ -140,3 +140,52 @@ def test_norm_of_a_step_without_gradients(options):
     opt.zero_grad()
     opt.step()
     assert float(opt.grad_norm) == 0.0 and torch.equal(p, after) and opt.device_state[0, 0] == 1.0
+
+
+# ---- captured clippings beyond the one-launch form ---------------------------------------------------------------------
+def test_captured_clippings_of_many_elements_on_two_streams():
+    """Lists that need partial sums, 300 tensors (two launches of sums and two of scaling), one of them strided: each graph has its
+    partial sums to itself, so two that replay at once do not disturb each other."""
+    sizes = [(1 + 37 * i % 900,) for i in range(298)] + [(3_000_000,)]
+    assert sum(s[0] for s in sizes) > NORM_SMALL_ELEMENTS
+    sets, graphs, norms = [], [], []
+
+    def fresh(seed, scale):
+        gen = torch.Generator(cuda()).manual_seed(seed)
+        return [scale * torch.empty(s, device=cuda()).normal_(generator=gen) for s in sizes + [(500, 3)]]
+    for k in range(2):
+        params = [torch.nn.Parameter(torch.zeros(s, device=cuda())) for s in sizes + [(500,)]]
+        wide = torch.zeros(500, 3, device=cuda())
+        for p in params[:-1]:
+            p.grad = torch.zeros_like(p)
+        params[-1].grad = wide[:, 1]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            clip_grad_norm_(params, 1.0)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norms.append(clip_grad_norm_(params, 1.0))
+        sets.append((params, wide))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for r in range(4):
+        given = [fresh(2 * r + k, 3.0 + k) for k in range(2)]
+        for (params, wide), grads in zip(sets, given):
+            for p, g in zip(params, grads[:-1]):
+                p.grad.copy_(g)
+            wide.copy_(grads[-1])
+        torch.cuda.synchronize()
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (params, wide), grads, norm in zip(sets, given, norms):
+            seen = grads[:-1] + [grads[-1][:, 1].contiguous()]
+            assert torch.equal(norm, grad_norm(seen))
+            want, factor = F.clip_factor([f64(g) for g in seen], 1.0)
+            assert abs(float(norm) / want - 1) <= 2 * H
+            for p, g in zip(params, seen):
+                assert (np.abs(f64(p.grad) - f64(g) * factor) <= 2 * H * np.abs(f64(g) * factor)).all()
+            assert torch.equal(wide[:, ::2], grads[-1][:, ::2])
