@@ -189,3 +189,52 @@ def test_captured_clippings_of_many_elements_on_two_streams():
             for p, g in zip(params, seen):
                 assert (np.abs(f64(p.grad) - f64(g) * factor) <= 2 * H * np.abs(f64(g) * factor)).all()
             assert torch.equal(wide[:, ::2], grads[-1][:, ::2])
+
+
+# ---- the largest 8-bit scales ----------------------------------------------------------------------------------------
+def held(x, first, t, form):
+    """one block as it is held in 8 bits, also where its values are beyond what the largest scale can hold: those take the largest code"""
+    tab = F.table(form)
+    a = np.abs(x)
+    scale = 0
+    while scale < form["most"] and a.max() >= tab[-1] * 2.0 ** (scale - 127):
+        scale += 1
+    y = a * 2.0 ** (127 - scale)
+    c = np.clip(np.searchsorted(tab, y, side="right") - 1, 0, len(tab) - 2)
+    i = np.arange(first, first + len(x), dtype=np.uint64)
+    word = (i * np.uint64(form["place"]) + np.uint64(t * form["step"] % 2 ** 32)) % np.uint64(2 ** 32)
+    u = ((word >> np.uint64(15)) | np.uint64(1)).astype(np.float64) / 2 ** 17
+    c = np.minimum(np.floor(c + (y - tab[c]) / (tab[c + 1] - tab[c]) + u), len(tab) - 1).astype(np.int64)
+    if form is F.V:
+        c = np.where(a > 0, np.maximum(c, 1), c)
+    return np.where(x < 0, -1.0, 1.0) * tab[c] * 2.0 ** (scale - 127), scale
+
+
+@pytest.mark.parametrize("scale", [1e18, 3e19, 1e21, 1e30, 7e37])
+def test_eight_bit_moments_at_their_largest(scale):
+    """exp_avg_sq holds 1.75 2^127 at most and exp_avg too: beyond, the largest code of the largest scale, in the blocks that need it alone.  Scales and
+    codes equal the formula's, and the weights follow the moments before they are rounded (at most 16 roundings)."""
+    n, lr = 1024, 1e-2
+    rng = np.random.default_rng(7)
+    p = torch.nn.Parameter(torch.zeros(n, device=cuda()))
+    opt = GroupedAdamW([p], lr=lr, weight_decay=0.0, state_bits=8)
+    m, v = np.zeros(n), np.zeros(n)
+    top = False
+    for t in range(1, 5):
+        g = rng.standard_normal(n) * scale
+        g[256:512] *= 1e-9
+        g[5] = 0.0
+        p.grad = on_gpu(g)
+        had = f64(p)
+        opt.step()
+        p1, m, v = F.step(had, f64(p.grad), m, v, t, lr, 0.9, 0.999, 1e-8, 0.0)
+        assert (np.abs(f64(p) - p1)[6:] <= 16 * H * (np.abs(p1 - had) + np.abs(p1))[6:]).all()
+        for x, form, codes, scales in ((m, F.M, opt.exp_avg, opt.exp_avg_scale), (v, F.V, opt.exp_avg_sq, opt.exp_avg_sq_scale)):
+            out = [held(x[b:b + 128], b, t, form) for b in range(0, n, 128)]
+            x[:] = np.concatenate([o[0] for o in out])
+            assert scales.cpu().tolist() == [o[1] for o in out], t
+            got = opt.moments()[0 if form is F.M else 1]
+            assert np.array_equal(f64(got), x), t
+            top |= form is F.V and max(o[1] for o in out) == form["most"] and int(codes.max()) == 254
+        assert torch.isfinite(p).all() and torch.isfinite(opt.moments()[1]).all()
+    assert top == (scale >= 1e21)                                             # (1 - b2) (3 scale)^2 against 3e38: 1e37 for 3e19, 1e40 for 1e21
