@@ -5,7 +5,7 @@
 //   p <- (1 - lr wd) p - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Every element is read and written once (28 bytes for float32 throughout), so the step is bound by memory: 240M float32 weights
-// 1.08 ms (6.2 TB/s; a copy of 4 GB by torch runs at 4.7), clipped 1.21 ms with the gradient read twice.  The tensors
+// 1.07 ms (6.3 TB/s; a plain copy kernel runs at 6.5), clipped 1.20 ms with the gradient read twice.  The tensors
 // are cut into chunks of 1024 or 2048 elements; a table that the caller keeps on the device says which tensor a chunk lies in, so
 // one launch covers up to kMaxTensors tensors of any sizes; their addresses travel in the launch's arguments, because
 // gradients move from step to step.  Moments and master weights are flat buffers in which each tensor starts at a multiple of kBlock.
@@ -18,8 +18,8 @@
 // The arithmetic is float64, whose products, sums and conversions issue as fast as integer operations here (4.4 to 5.4 cycles a
 // wave; float32 additions 2.8): the top 20 bits of a double's mantissa hold the 3 bits of the code and 17 bits of remainder, so
 // rounding is one integer addition on the double's upper word, and it is exact - the codes do not depend on how a compiler
-// contracts a float32 expression.  240M weights: float32 660 us (16 bytes each, 5.8 TB/s), bfloat16 440 us (10 bytes, 5.5 TB/s: its 52
-// vector instructions an element, 360 us of issue, no longer hide under 387 us of memory).
+// contracts a float32 expression.  60M float32 weights 171 us (16 bytes each, 5.6 TB/s), 240M bfloat16 weights 440 us (10 bytes, 5.5 TB/s:
+// 56 vector instructions an element, 383 us of issue, no longer hide under 370 us of memory).
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -669,7 +669,7 @@ __device__ inline void chunk_scale(T *x, int count, Factor f)
     if (i < count) x[i] = (T)(f * (float)x[i]);
 }
 
-// 240M float32 elements, norm and scaling: 472 us (2.88 GB, 6.1 TB/s); where the norm is small enough nothing is scaled: 143 us.  The
+// 240M float32 elements, norm and scaling: 478 us (2.88 GB, 6.0 TB/s); where the norm is small enough nothing is scaled: 143 us.  The
 // workgroups of the sums take the chunks in turn: one for each chunk scales 240M bfloat16 elements in 170 us instead of 181 (float32 336
 // and 365), but where nothing is to be scaled, which only the kernel knows, they take 26 us to start and leave, not 4.6.
 __global__ __launch_bounds__(kThreads) void k_grad_clip(const NormArgs a, const double *partials, int n_partials, double max_norm, float *norm_out)
@@ -763,7 +763,7 @@ void launch_step(const StepArgs &a, StepConst c, int bits, hipStream_t st)
 {
     // 10 bytes an element (8-bit moments, 16-bit weights without masters) leave so little to wait for that the instructions count: such
     // workgroups take 4 chunks each, which spreads the scalars of a step over more elements, and are not held back.  240M bfloat16
-    // weights: 1 chunk 518 us, 2 451, 4 432, 8 446; held to 5 workgroups 560.  All others are bound by memory and go fastest when workgroups
+    // weights: 1 chunk 518 us, 2 451, 4 432, 8 446; held to 5 workgroups 560 (lists that do not fill the card have not been compared).  All others are bound by memory and go fastest when workgroups
     // come and go in the order of the addresses: 240M float32 weights, 8-bit moments: 1 chunk 773 us, 2 854, 4 957.
     const bool lean = bits == 8 && sizeof(T) == 2 && !MASTER;
     c.run = lean ? 4 : 1;

@@ -306,7 +306,7 @@ class GroupedAdamW(torch.optim.Optimizer):
     state_bits      32: moments in float32.  8: one byte each, in blocks of 128 elements with a power-of-two scale (2 1/64 bytes
                     per weight instead of 8): exp_avg keeps 4 significant bits and a range of 2^17 in a block, exp_avg_sq 4 bits and 2^33;
                     rounded by an even sequence, so that small changes are not lost.  Both hold 1.75 * 2^127 at most: an exp_avg_sq
-                    beyond (gradients above about 5e20) stays at that.  A gradient that is not finite makes its whole block's moments NaN.
+                    beyond (gradients above 1.7e19 that last) stays at that.  A gradient that is not finite makes its whole block's moments NaN.
     max_norm        clip the gradients' global 2-norm (over all groups, tensors without a gradient left out) inside the step; the gradients themselves
                     stay as they are.  `grad_norm` holds the norm of the last step, on the device.
     skip_nonfinite  a step whose gradient norm is not finite, as `grad_norm` gives it, changes nothing, counters included (decided on the device).
