@@ -162,7 +162,7 @@ int pinn_loss_grad(pinn_handle *h, const float *theta, const float *x, const flo
                    int64_t stride, int64_t n, float scale, float *loss_sums_accum,
                    float *grad_theta_accum, void *stream);
 
-/* ---- L-BFGS on the device --------------------------------------------------
+/* ---- L-BFGS on the device ------------------------------------------------------------------
  * The reference ends every run with torch.optim.LBFGS.step(closure), strong-Wolfe
  * (7kdv/PI-7kdv3soliton.py:138-161; third-party torch/optim/lbfgs.py).  These two entry points
  * replace that optimizer's per-iteration tensor work with one launch each; the line search's
@@ -244,7 +244,7 @@ int pinn_data_loss_cotangent(const float *out, const float *tgt0, int32_t n0, in
 int pinn_closure_sum(const float *terms, int32_t n_terms, float *sums, int32_t nf, float n_total, float *loss2,
                      const float *ga, float *gb, float *grad, int64_t P, int32_t flags, void *stream);
 
-/* ---- Adam / AdamW on the device, one launch per step ------------------------------------
+/* ---- Adam / AdamW on the device, one launch per step ----------------------------------------------------
  * Replaces torch.optim.Adam / AdamW(weight_decay=1e-2).step() of the reference's Adam phase
  * (7kdv/PI-7kdv3soliton.py:138,154-157; 7kdv/sw73-adamW.py:170) for parameters held as ONE flat vector:
  * the arithmetic of torch's default (non-amsgrad) Adam, decoupled != 0 selects AdamW's decay.  `state` is

@@ -1,4 +1,4 @@
-// Fused Adam / AdamW step over the flat parameter vector (SURVEY 8(f)-1).
+// Fused Adam / AdamW step over the flat parameter vector.
 //
 // The reference's Adam phase is torch.optim.Adam / AdamW(weight_decay=1e-2) on the ten parameter tensors of the
 // net (7kdv/PI-7kdv3soliton.py:138,154-157; 7kdv/sw73-adamW.py:170).  torch runs it as ~15 foreach launches per

@@ -22,7 +22,7 @@ template <int EQ> struct EqTraits;
 // evaluated in float64.  For Camassa-Holm: f = (u - u_xx)_t + ... is a cancellation of u_xxt against u u_xxx
 // (~1500 against ~1400 at the crest of the trained peakon) whose two sides come out of DIFFERENT jet components,
 // i.e. different float32 dot products with independent rounding errors, while the reference's nested-autograd
-// graph perturbs both consistently.  Stage by stage (tools/ch_noise_lab.py, DESIGN.md section 2) the excess noise
+// graph perturbs both consistently.  Stage by stage (tools/ch_noise_lab.py) the excess noise
 // sits in exactly those late dot products: made exact, the residual / loss / gradient noise at CH/model/PINN CH.pth
 // falls from 3.4x / 4.8x / 5.7x the reference's own fp32 noise to 1.3x / 1.5x / 1.5x (96 batches of 256 points).
 // It is on for every residual: at the other seven shipped checkpoints it takes the noise from 0.7-1.8x the
@@ -43,12 +43,12 @@ constexpr int MAXF = 3;     // residual components per point: two outputs + one 
 
 // tanh(x) and w0 = 1 - tanh(x)^2 = sech(x)^2, both to ~1 ulp, branch-free.
 //
-// Why not exp-based (1 - e)/(1 + e) with the hardware v_exp_f32 (what round 1 shipped): e carries >= 1 ulp
+// Why not exp-based (1 - e)/(1 + e) with the hardware v_exp_f32: e carries >= 1 ulp
 // of ABSOLUTE error near 1, which 1 - e turns into several ulp of tanh for |x| in [0.04, 0.3], and
 // w0 = 1 - y^2 then inherits 2|y| ulp(1) of absolute error however small w0 is.  At trained weights the
 // PDE residual is a ~1000x cancellation of terms that are all linear in these two numbers, and the extra
 // ulps showed up as 2-3x the residual / gradient noise of the reference's own fp32 run
-// (DESIGN.md section 2; oracle variants: a +2 ulp bias in tanh alone gives 2-8x).
+// (oracle variants: a +2 ulp bias in tanh alone gives 2-8x).
 //
 // Here: a = -2|x| = n ln2 + r, |r| <= ln2/2;  p = expm1(r) by its Taylor polynomial through r^8/8!
 // (relative error < 0.3 ulp, r is exact for n = 0);  e = exp(a) = s (1 + p), s = 2^n.  Then
@@ -60,7 +60,7 @@ __device__ __forceinline__ float tanh_sech2(float x, float &w0)
 {
     // |x| > 22: tanh = 1 and sech^2 < 4 e^-44 = 3e-19 in float.  The ARGUMENT is clamped (a select, so that NaN
     // stays NaN), not just the exponent: with only n clamped the remainder r = a - n ln2 of a large |x| is not
-    // small, the expm1 polynomial blows up and tanh(500) came out as 0.04 (round-2 regression).
+    // small, the expm1 polynomial blows up and tanh(500) came out as 0.04.
     const float ax0 = fabsf(x);
     const float ax = ax0 > 22.0f ? 22.0f : ax0;
     const float a = -2.0f * ax;

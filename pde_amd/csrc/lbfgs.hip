@@ -1,4 +1,4 @@
-// L-BFGS search direction on the device (SURVEY 8(f)-1).
+// L-BFGS search direction on the device.
 //
 // The reference finishes every training run with one torch.optim.LBFGS.step(closure)
 // (7kdv/PI-7kdv3soliton.py:138-161) of up to 50 000 closure evaluations.  torch's

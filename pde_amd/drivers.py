@@ -1,5 +1,5 @@
 """The reference's sw- (sliding time window) and bc- (backward-compatible) training drivers as
-library functions (SURVEY 8(f)-3), with the small pieces of data preparation they need.
+library functions, with the small pieces of data preparation they need.
 
 In the reference these loops live in each script's ``__main__`` (``7kdv/sw-73.py:264-380``,
 ``CH/bc-CH-1soliton.py:378-473``); here they are functions of (model classes, grid data, sizes), so a
@@ -24,7 +24,7 @@ def lhs(n, samples, rng=None):
 
 
 def lhs_device(n, samples, device, generator=None, dtype=None):
-    """`lhs` generated on `device` as a torch tensor (SURVEY 8(f)-3: the 10M-point CH configuration would
+    """`lhs` generated on `device` as a torch tensor (the 10M-point CH configuration would
     otherwise spend seconds in numpy permutations and ship 160 MB over PCIe per resampling).  Same
     construction: one point per stratum and coordinate, uniformly placed, strata paired at random.
     `set_training_data` accepts the result (after scaling to the domain) as `Xf` without a host copy."""

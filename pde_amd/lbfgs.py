@@ -1,4 +1,4 @@
-"""L-BFGS with strong-Wolfe line search whose vector work stays on the GPU (SURVEY 8(f)-1).
+"""L-BFGS with strong-Wolfe line search whose vector work stays on the GPU.
 
 Every reference script ends `train()` with ONE `torch.optim.LBFGS(...).step(closure)` of up to
 50 000 closure evaluations (7kdv/PI-7kdv3soliton.py:138-161) — at the scripts' own sizes that is

@@ -56,7 +56,7 @@ class FileWriter:
 @dataclass
 class Variant:
     equation: str = "kdv7_3sol"
-    t0: float = -0.5                 # IC time literal (SURVEY 8(a) quirks)
+    t0: float = -0.5                 # IC time literal
     bc: str = "periodic"             # "periodic" (:105) or "dirichlet" (Burgers :109)
     style: str = "pi"                # "pi" | "sw" | "bc"  (set_training_data signature, extra loss term)
     optimizer: str = "adam"          # "adam" | "adamw"
@@ -77,7 +77,7 @@ class PhysicsInformedNN:
     kernel = KERNEL_AUTO
     use_hip_graph = False            # train(): replay the Adam phase / the L-BFGS closure from a captured HIP graph
     # eager backward(): the collocation kernel on a second stream beside the data-term chain.  None = automatic: when
-    # that kernel is long enough to pay for the host work of two streams, N_f x P >= 1e8 (round 3, eager Adam steps/s
+    # that kernel is long enough to pay for the host work of two streams, N_f x P >= 1e8 (eager Adam steps/s
     # with / without: 7kdv at 20 000 points 3 877 / 3 194, GNSS-100 1 841 / 1 365, but Burgers 4x50 at 10 000 points
     # 4 940 / 5 202 and Burgers 8x20 4 733 / 7 018: closures that short are host-bound)
     overlap_streams = None
@@ -138,7 +138,7 @@ class PhysicsInformedNN:
 
     def _shard(self, Xf):
         """Contiguous equal shards of the collocation points over the ranks of the
-        process group (SURVEY 8(e)); remainder goes to the low ranks."""
+        process group; remainder goes to the low ranks."""
         if not torch.is_tensor(Xf):
             Xf = np.asarray(Xf)
         self.n_f_global = Xf.shape[0]
@@ -460,7 +460,7 @@ class PhysicsInformedNN:
     _T_SUMS, _T_L0, _T_L1, _T_LPREV, _T_LS, _T_SIZE = 0, 3, 5, 7, 9, 10
 
     def _loss_terms_sharded(self, data_terms=True):
-        """The closure of a sharded run (SURVEY 8(e)): every rank evaluates the collocation term on ITS
+        """The closure of a sharded run: every rank evaluates the collocation term on ITS
         shard (gradient already scaled by 1/N_global), rank 0 alone evaluates the data terms
         (IC, boundary, loss1, loss_prev, loss_s: at most a few thousand points), and ONE all-reduce(SUM) of
         [flat gradient (P) | sum_p f_c^2 (3) | loss0, loss_b | loss1 | loss_prev | loss_s] gives every rank the
@@ -759,7 +759,7 @@ class PhysicsInformedNN:
         return self.closure_impl == "direct" and dist.get_backend(self.group) == "nccl"
 
     def _train_adam_graph(self, nIter, params):
-        """the Adam phase without per-iteration host work.  One whole iteration
+        """The Adam phase without per-iteration host work.  One whole iteration
         (zero_grad, the loss terms, loss.backward(), Adam(capturable).step()) is captured into a HIP
         graph after a few eager iterations and replayed; the host only touches the device for the
         reference's every-100-iterations log line.  Same kernels in the same order as the eager loop

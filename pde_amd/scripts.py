@@ -4,9 +4,9 @@ Usage inside a reference script: delete its Scale/DNN/PhysicsInformedNN class
 definitions and write e.g.
     from pde_amd import scripts
     PhysicsInformedNN = scripts.for_script("7kdv/sw-73.py").PhysicsInformedNN
-(see INTEGRATION.md).  What differs from script to script is a literal table: the
-residual body, the IC time `t0` (SURVEY 8(a) quirks), the boundary-loss form, Adam vs
-AdamW, the L-BFGS settings (SURVEY a9).  Every row below cites the reference lines it was
+What differs from script to script is a literal table: the
+residual body, the IC time `t0`, the boundary-loss form, Adam vs
+AdamW, the L-BFGS settings.  Every row below cites the reference lines it was
 read from, and tests/test_host_logic.py::test_script_literals_match_reference compares the
 whole table with tests/golden/script_literals.json, which oracle/gen_script_literals.py
 extracts from the reference's source text.
@@ -135,7 +135,7 @@ nls = _family(sw="NLS/sw-PINN-rogue.py")
 lpd = _family(bc="NLS/Ibc-test.py")
 nls_reg = _family(sw="NLS/sw-test.py")
 
-# flat aliases used in INTEGRATION.md
+# flat aliases
 kdv7_3soliton_PI = kdv7_3soliton.PI
 kdv7_3soliton_sw = kdv7_3soliton.sw
 kdv7_3soliton_sw_adamW = kdv7_3soliton.sw_adamW
