@@ -83,8 +83,9 @@ def _layout():
     def of_struct(s):
         return of(ctypes.sizeof(s), [(name, getattr(s, name).offset) for name, _ in s._fields_])
     chunk = of(ADAMW_CHUNK_DTYPE.itemsize, [(name, ADAMW_CHUNK_DTYPE.fields[name][1]) for name in ADAMW_CHUNK_DTYPE.names])
-    return of_struct(PinnDesc) + chunk + of_struct(PinnAdamWGroup) + [ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_MAX_TENSORS, ADAMW_MAX_CHUNKS, ADAMW_TICKET_WORDS,
-                                      NORM_SMALL_TENSORS, NORM_SMALL_ELEMENTS, ERR_OVERLAP]
+    constants = [ADAMW_BLOCK, ADAMW_CHUNK32, ADAMW_CHUNK8, ADAMW_MAX_TENSORS, ADAMW_MAX_CHUNKS, ADAMW_TICKET_WORDS,
+                 NORM_SMALL_TENSORS, NORM_SMALL_ELEMENTS, ERR_OVERLAP]
+    return of_struct(PinnDesc) + chunk + of_struct(PinnAdamWGroup) + constants
 
 
 def _check_library(lib):

@@ -48,6 +48,13 @@ def test_build_compiles_every_unit_every_time(monkeypatch):
     assert sorted(ran) == sorted((name, True) for name in units + ["libpinnjet.so", "_tensorlist.so"])
 
 
+def test_development_builds_have_every_unit():
+    """tools/dev_build.sh links what it builds of pinnjet.hip with all the others: load_library takes no library with an entry point missing"""
+    script = open(os.path.join(ROOT, "tools", "dev_build.sh")).read()
+    named = set(script.split("for unit in ")[1].split(";")[0].split()) | {"pinnjet"}
+    assert named == {f[:-4] for f in os.listdir(os.path.join(ROOT, "pde_amd", "csrc")) if f.endswith(".hip")}
+
+
 @pytest.mark.skipif(not os.path.exists(os.path.join(ROOT, "pde_amd", "_tensorlist.so")), reason="_tensorlist.so not built")
 def test_a_list_reader_for_another_torch_is_noticed(monkeypatch):
     assert native.load_tensorlist().torch_version == str(torch.__version__)

@@ -6,10 +6,16 @@ set -e
 cd "$(dirname "$0")/.."
 name=$1; shift
 mkdir -p build_dev/$name
-flags="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-slp-vectorize -DPINN_WITH_MFMA -DPINN_DEV_${WHICH:-KDV7}_ONLY"
+flags="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fno-slp-vectorize -Xclang -target-feature -Xclang -packed-fp32-ops -DPINN_WITH_MFMA -DPINN_DEV_${WHICH:-KDV7}_ONLY"
 /opt/rocm/bin/hipcc $flags "$@" -save-temps=obj -c pde_amd/csrc/pinnjet.hip -o build_dev/$name/pinnjet.o
-[ -f build_obj/lbfgs.hip.o ] || /opt/rocm/bin/hipcc $flags -c pde_amd/csrc/lbfgs.hip -o build_obj/lbfgs.hip.o
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC build_dev/$name/pinnjet.o build_obj/lbfgs.hip.o build_obj/adam.hip.o build_obj/dataloss.hip.o -o build_dev/lib_$name.so
+mkdir -p build_obj
+objs=""
+for unit in lbfgs adam dataloss adamw_group; do    # every other unit: the package refuses a library without all of them
+  obj=build_obj/$unit.hip.o
+  { [ -f $obj ] && [ $obj -nt pde_amd/csrc/$unit.hip ] && [ $obj -nt include/pinnjet.h ]; } || { rm -f $obj.cmd; /opt/rocm/bin/hipcc $flags -c pde_amd/csrc/$unit.hip -o $obj; }
+  objs="$objs $obj"
+done
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC build_dev/$name/pinnjet.o $objs -o build_dev/lib_$name.so
 s=$(ls build_dev/$name/*gfx950*.s | head -1)
 grep -A40 "k_mfmaILi3ELi50ELi2E" $s | grep -m1 -A30 "\.amdhsa_kernel\|; Kernel info" >/dev/null 2>&1 || true
 python3 - "$s" <<'PY'
