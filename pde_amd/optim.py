@@ -349,6 +349,10 @@ class GroupedAdamW(torch.optim.Optimizer):
             raise ValueError("GroupedAdamW takes all parameter groups when it is made")
         super().add_param_group(param_group)
 
+    def __getstate__(self):
+        # torch's would leave out the moments and the tables, all that is not in `state`
+        raise TypeError("GroupedAdamW cannot be copied or pickled: make another and load_state_dict(state_dict())")
+
     @staticmethod
     def _hyper(grp):
         lr, (b1, b2), eps, wd = float(grp["lr"]), grp["betas"], float(grp["eps"]), float(grp["weight_decay"])

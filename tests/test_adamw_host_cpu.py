@@ -1,6 +1,8 @@
 """CPU: the host side of GroupedAdamW, grad_norm and clip_grad_norm_ - arguments that would be taken for others, parameter lists without
 a parameter, gradients that share memory, libraries that do not fit this package."""
+import copy
 import os
+import pickle
 
 import numpy as np
 import pytest
@@ -25,6 +27,14 @@ def test_a_norm_type_is_not_taken_for_error_if_nonfinite(third):
 def test_groups_without_any_parameter_are_refused():
     with pytest.raises(ValueError, match="no parameter"):
         GroupedAdamW([dict(params=[]), dict(params=[])])
+
+
+def test_copies_that_would_lose_the_moments_are_refused():
+    opt = object.__new__(GroupedAdamW)
+    opt.__dict__.update(defaults={}, state={}, param_groups=[], exp_avg=torch.ones(3))
+    for call in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="load_state_dict"):
+            call(opt)
 
 
 def columns(rows, n, dtype=torch.float32):
