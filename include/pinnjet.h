@@ -263,7 +263,8 @@ int pinn_adam_step(float *theta, const float *grad, float *exp_avg, float *exp_a
  * Moments, master weights and scales are flat device buffers in which every tensor starts at a multiple of
  * PINN_ADAMW_BLOCK elements; the elements behind a tensor's end are not written to (8 bits: they hold 0).
  * 8-bit moments: one scale byte s per block, 2^(s - 127), 255 = the block holds a value that is not finite (it reads NaN
- * from then on), 246 at most for exp_avg and 238 for exp_avg_sq, so that no value passes 1.75 * 2^127: a larger moment is held as that; exp_avg: sign, 4 bits of exponent (bias 7), 3 of mantissa; exp_avg_sq: 5 bits of exponent (bias 15), 3 of mantissa.
+ * from then on), 246 at most for exp_avg and 238 for exp_avg_sq, so that no value passes 1.75 * 2^127: a larger moment is held as that;
+ * exp_avg: sign, 4 bits of exponent (bias 7), 3 of mantissa; exp_avg_sq: 5 bits of exponent (bias 15), 3 of mantissa.
  * They are formed in float64, each operation rounded by itself; on the scale of the codes (equal steps between neighbours, y a float64) the
  * code is floor(y + u), u in (0, 1) from a sequence over steps and elements that is even on both sides; a positive v never becomes 0.
  * No entry point here allocates or synchronises: all are graph-capturable.  pinn_adamw_group_step must not run twice at
@@ -332,9 +333,9 @@ int pinn_grad_clip(void *const *grads, const int64_t *numel, const int32_t *dtyp
 
 const char *pinn_error_string(int code);
 
-/* What a caller's structs and tables are laid out by, for one that was compiled apart from the library to compare: writes the first n of these
- * and returns how many there are.  sizeof pinn_desc and for each of its fields the name's 32-bit FNV-1a hash and the offset, the same of PinnAdamWChunk and PinnAdamWGroup, then PINN_ADAMW_BLOCK,
- * _CHUNK32, _CHUNK8, _MAX_TENSORS, _MAX_CHUNKS, _TICKET_WORDS, PINN_NORM_SMALL_TENSORS, _SMALL_ELEMENTS, PINN_ERR_OVERLAP. */
+/* What a caller's structs and tables are laid out by, for one that was compiled apart from the library to compare: writes the first n of
+ * these and returns how many there are.  sizeof pinn_desc and for each of its fields the name's 32-bit FNV-1a hash and the offset, the same
+ * of PinnAdamWChunk and PinnAdamWGroup, then PINN_ADAMW_BLOCK, _CHUNK32, _CHUNK8, _MAX_TENSORS, _MAX_CHUNKS, _TICKET_WORDS, PINN_NORM_SMALL_TENSORS, _SMALL_ELEMENTS, PINN_ERR_OVERLAP. */
 int32_t pinn_layout(int32_t *out, int32_t n);
 
 #define PINN_OK 0
